@@ -535,6 +535,74 @@ int32_t izb_paged_decode_gqa_attention(izb_ctx* ctx, izb_stream stream, const vo
                                        int64_t batch, int32_t heads, int64_t max_seq_len, int64_t ld_q,
                                        int64_t ld_out, float scale, void* workspace, size_t workspace_bytes);
 
+/* ---- beam search ------------------------------------------------------------------------------------
+ * Several continuations (beams) of each of `groups` sequences are decoded together; beam b of group g is
+ * sequence g * beams + b.  A step is: logits of all beams -> izb_beam_select -> izb_kv_pages_reorder ->
+ * the next token.  Beams share the pages of their prompt (izb_shared_prefix_decode_gqa_attention) and own
+ * pages for what they add.  The reference decodes one continuation per sequence and has no counterpart to
+ * cite for these four. */
+
+/* The n_out best extensions of every group's beams: total(b, v) = scores[b] + logits[b, v] - lse_b with
+ * lse_b = log sum exp over the finite logits of beam b, in descending order of total, equal totals in
+ * ascending order of b * vocab + v.  Candidates are ranked in fp64 and scores_out rounded once.
+ *   logits [groups * beams, vocab] bf16 / fp32 / fp16, rows ld apart (any alignment of whole elements);
+ *   non-finite logits are never chosen;
+ *   scores [groups, beams] fp32: log-probability of each beam so far.  A beam whose score is not finite has
+ *   no extension (the first step: 0 for one beam, -inf for the others) and its row is not read;
+ *   finished [groups, beams] bytes or NULL: a finished beam has one extension, the token eos at its own
+ *   score, and its row is not read.  eos: -1 for none (then finished must be NULL).
+ * scores_out, parents_out (beam inside the group), tokens_out, finished_out (may be NULL; 1 where the parent
+ * is finished or the token is eos): [groups, n_out].  Places without a candidate get score -inf, parent 0,
+ * token eos (0 without one), finished 0.  With n_out == beams, scores_out may be scores and finished_out may
+ * be finished.  beams <= 32, n_out <= 64. */
+size_t izb_beam_select_workspace_bytes(const izb_ctx* ctx, int32_t dtype, int64_t groups, int32_t beams,
+                                       int64_t vocab, int32_t n_out);
+int32_t izb_beam_select(izb_ctx* ctx, izb_stream stream, const void* logits, int32_t dtype, int64_t groups,
+                        int32_t beams, int64_t vocab, int64_t ld, const float* scores, const uint8_t* finished,
+                        int32_t eos, int32_t n_out, float* scores_out, int32_t* parents_out,
+                        int32_t* tokens_out, uint8_t* finished_out, void* workspace, size_t workspace_bytes);
+/* Makes beam k of every group continue what beam parents[k] of the group has cached, in all layers at once.
+ * layers: HOST array [n_layers <= 64] of page descriptors that name one page table [groups * beams,
+ * max_pages_per_seq] and agree in everything but their buffers; the pages of a group's beams that are not
+ * full yet must be distinct.  seq_lens [groups * beams]: tokens cached, the same for the beams of a group.
+ * page_table_out (not overlapping the old table) receives the table to use from now on: entries of filled
+ * pages are copied from the parent; the partly filled page goes on with the parent's first child, and
+ * further children get the pages of beams that have no child, into which the rows held so far (and their
+ * scales) are copied; later entries stay.  parents [groups * beams] int32, each in [0, beams).  A group with a parent
+ * outside that range, unequal lengths or a length beyond its table keeps its rows unchanged and makes the
+ * next izb_ctx_check return IZB_ERR_BAD_ARG.  beams <= 32. */
+int32_t izb_kv_pages_reorder(izb_ctx* ctx, izb_stream stream, const izb_kv_pages* layers, int32_t n_layers,
+                             const int32_t* parents, int64_t groups, int32_t beams, const int32_t* seq_lens,
+                             int32_t* page_table_out);
+/* Token sequences of chosen beams, walked back through the steps' choices: out[g, j, s] = tokens[s, g, b_s]
+ * with b_{s-1} = parents[s, g, b_s] and b = last[g, j] at the last step.  parents / tokens
+ * [steps, groups, beams] int32, last [groups, picks] int32, out rows ld_out apart.  A beam index outside
+ * [0, beams) on the way leaves -1 from that step down and makes the next izb_ctx_check return
+ * IZB_ERR_BAD_ARG. */
+int32_t izb_beam_trace(izb_ctx* ctx, izb_stream stream, const int32_t* parents, const int32_t* tokens,
+                       int64_t steps, int64_t groups, int32_t beams, const int32_t* last, int32_t picks,
+                       int32_t* out, int64_t ld_out);
+/* One query token per sequence over a prefix that the sequences of a group share and then over pages of
+ * their own: sequence g * seqs_per_group + j attends to the prefix_lens[g] tokens of row g of `prefix` and
+ * the seq_lens[...] tokens of its row of `pages` (NULL with max_seq_len 0: the prefix alone, as in
+ * cross-attention of several beams over one encoder output), out = softmax(q k^T * scale) v over both.
+ * The prefix is read once for all sequences of its group.  Both caches have the same kv_heads and head_dim
+ * (64 or 128); storage and page size may differ.  q / out [groups * seqs_per_group, heads, head_dim] bf16,
+ * rows ld_q / ld_out apart, q 16-byte aligned rows; heads / kv_heads <= 16.  Lengths are device int32,
+ * cut to [0, max_prefix_len] and [0, max_seq_len], which the page tables must cover (IZB_ERR_BAD_ARG);
+ * a sequence without any token gives zeros. */
+size_t izb_shared_prefix_decode_gqa_attention_workspace_bytes(const izb_ctx* ctx, int64_t groups,
+                                                              int64_t seqs_per_group, int32_t heads,
+                                                              int32_t kv_heads, int32_t head_dim,
+                                                              int64_t max_prefix_len, int64_t max_seq_len);
+int32_t izb_shared_prefix_decode_gqa_attention(izb_ctx* ctx, izb_stream stream, const void* q,
+                                               const izb_kv_pages* prefix, const int32_t* prefix_lens,
+                                               const izb_kv_pages* pages, const int32_t* seq_lens, void* out,
+                                               int64_t groups, int64_t seqs_per_group, int32_t heads,
+                                               int64_t max_prefix_len, int64_t max_seq_len, int64_t ld_q,
+                                               int64_t ld_out, float scale, void* workspace,
+                                               size_t workspace_bytes);
+
 /* ---- what a prompt needs before the first decode step -----------------------------------------
  * out[t, :] = table[ids[t], :]: the embedding lookup in front of the first layer (`embed_tokens`,
  * models/architectures/qwen3/core.rs:2099-2103).  table bf16 [vocab, hidden], ids int32 on the device

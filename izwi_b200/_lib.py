@@ -172,6 +172,20 @@ _SIGNATURES = {
     "izb_paged_decode_gqa_attention": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(KvPages), C.c_void_p, C.c_void_p,
                                                    C.c_int64, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_float, C.c_void_p,
                                                    C.c_size_t]),
+    "izb_beam_select_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_int32]),
+    "izb_beam_select": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_int64, C.c_void_p,
+                                    C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                    C.c_size_t]),
+    "izb_kv_pages_reorder": (C.c_int32, [C.c_void_p, C.c_void_p, C.POINTER(KvPages), C.c_int32, C.c_void_p, C.c_int64, C.c_int32,
+                                         C.c_void_p, C.c_void_p]),
+    "izb_beam_trace": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_void_p,
+                                   C.c_int32, C.c_void_p, C.c_int64]),
+    "izb_shared_prefix_decode_gqa_attention_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_int32,
+                                                                           C.c_int32, C.c_int64, C.c_int64]),
+    "izb_shared_prefix_decode_gqa_attention": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(KvPages), C.c_void_p,
+                                                           C.POINTER(KvPages), C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int32,
+                                                           C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_float, C.c_void_p,
+                                                           C.c_size_t]),
     "izb_embed_rows": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
                                    C.c_int64]),
     "izb_qk_norm_rope_append_seq": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_float,

@@ -1,0 +1,628 @@
+// Beam search on the device: the choice of the next beams from the logits, the reordering of the paged caches that
+// follows it, and the walk back through the choices at the end.
+#include <climits>
+#include <type_traits>
+
+#include "izb_common.cuh"
+
+namespace {
+
+// ---- selection -----------------------------------------------------------------------------------------------------
+//   total(b, v) = score_b + logit_bv - lse_b,  lse_b = log sum over the finite logits of beam b of exp
+// and the n_out largest totals of a group's beams, equal ones in the order of b * vocab + v.
+//
+// Inside a row the order is that of the logits, so one pass over them yields, for every tile of a row, the tile's
+// maximum, its sum of exp(x - maximum) and its n_out largest (value, index) pairs; a second launch forms lse_b from
+// the tiles, the totals of the few pairs that are left (in fp64: candidates of different beams are ranked by them),
+// and their order.  Bound by reading the logits once.
+
+constexpr int BS_THREADS = 256;
+constexpr int BS_WARPS = BS_THREADS / 32;
+constexpr int BS_MAX_BEAMS = 32;
+constexpr int BS_MAX_OUT = 64;
+constexpr int BS_CAP = 1024;  // candidates kept in shared memory at a time
+
+using u64 = unsigned long long;
+
+// larger value <-> larger key, -0 as +0
+__device__ __forceinline__ uint32_t key_of(float v) {
+    const uint32_t u = __float_as_uint(v + 0.0f);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k); }
+__device__ __forceinline__ u64 key_of(double v) {
+    const u64 u = static_cast<u64>(__double_as_longlong(v + 0.0));
+    return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
+}
+__device__ __forceinline__ double value_of(u64 k) {
+    return __longlong_as_double(static_cast<long long>((k >> 63) ? (k & 0x7FFFFFFFFFFFFFFFull) : ~k));
+}
+
+// The k-th largest of the 32 lanes' keys (k <= 32).
+__device__ __forceinline__ u64 warp_kth(u64 key, int k) {
+    const int lane = threadIdx.x & 31;
+    int rank = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const u64 other = __shfl_sync(0xFFFFFFFFu, key, i);
+        rank += other > key || (other == key && i < lane);
+    }
+    const unsigned hit = __ballot_sync(0xFFFFFFFFu, rank == k - 1);
+    return __shfl_sync(0xFFFFFFFFu, key, __ffs(hit) - 1);
+}
+
+// A bound below which none of the k largest keys can lie, from every thread's largest key: the k-th largest lane of
+// any warp is such a bound (k <= 32), for more keys the smaller bound of two warps that give half of them each.
+// `slots` holds one key per warp; every thread returns the largest bound.
+__device__ __forceinline__ u64 block_bound(u64 mine, int k, u64* slots) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const u64 w = warp_kth(mine, k <= 32 ? k : (k + 1) / 2);
+    if (lane == 0) slots[warp] = w;
+    __syncthreads();
+    u64 bound = 0;
+#pragma unroll
+    for (int i = 0; i < BS_WARPS; i += 2) {
+        const u64 a = slots[i], b = slots[i + 1];
+        const u64 x = k <= 32 ? (a > b ? a : b) : (a < b ? a : b);
+        bound = x > bound ? x : bound;
+    }
+    return bound;
+}
+
+// Candidates in shared memory: a key and, among equal keys, the lower index first.
+struct Pool {
+    u64 key[BS_CAP];
+    uint32_t idx[BS_CAP];
+    unsigned count;
+};
+__device__ __forceinline__ bool before(u64 ka, uint32_t ia, u64 kb, uint32_t ib) { return ka > kb || (ka == kb && ia < ib); }
+
+__device__ __forceinline__ void pool_add(Pool& p, u64 key, uint32_t idx) {
+    const unsigned at = atomicAdd(&p.count, 1u);
+    if (at < BS_CAP) {
+        p.key[at] = key;
+        p.idx[at] = idx;
+    }
+}
+// Descending order over the first n entries (n <= BS_CAP), by bitonic exchange over the next power of two.
+__device__ void pool_sort(Pool& p, int n) {
+    int size = 2;
+    while (size < n) size <<= 1;
+    for (int i = n + threadIdx.x; i < size; i += BS_THREADS) {
+        p.key[i] = 0;
+        p.idx[i] = 0xFFFFFFFFu;
+    }
+    __syncthreads();
+    for (int block = 2; block <= size; block <<= 1)
+        for (int step = block >> 1; step > 0; step >>= 1) {
+            for (int i = threadIdx.x; i < size / 2; i += BS_THREADS) {
+                const int a = 2 * i - (i & (step - 1)), b = a + step;
+                const bool down = (a & block) == 0;
+                const u64 ka = p.key[a], kb = p.key[b];
+                const uint32_t ia = p.idx[a], ib = p.idx[b];
+                if (before(kb, ib, ka, ia) == down) {
+                    p.key[a] = kb; p.idx[a] = ib;
+                    p.key[b] = ka; p.idx[b] = ia;
+                }
+            }
+            __syncthreads();
+        }
+}
+
+// Fills the pool with every candidate not behind (bound_key, bound_idx); when they outgrow it, the k-th of those it
+// caught is a tighter bound (any k candidates bound the k largest), and the scan is repeated: each repetition drops
+// at least BS_CAP - k candidates for good.  Then sorts.  Returns the number of sorted entries, at least the k
+// largest if there are that many.  `scan(key, idx)` calls add for every candidate not behind the bound.
+template <typename Scan>
+__device__ int collect(Pool& p, u64 bound_key, int k, Scan scan) {
+    uint32_t bound_idx = 0xFFFFFFFFu;
+    for (;;) {
+        __syncthreads();
+        if (threadIdx.x == 0) p.count = 0;
+        __syncthreads();
+        scan(bound_key, bound_idx);
+        __syncthreads();
+        const unsigned n = p.count;
+        pool_sort(p, n < BS_CAP ? n : BS_CAP);
+        if (n <= BS_CAP) return static_cast<int>(n);
+        bound_key = p.key[k - 1];
+        bound_idx = p.idx[k - 1];
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ float element(const uint4& w, int i) {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    if constexpr (sizeof(T) == 4) {
+        return __uint_as_float(x[i]);
+    } else {
+        const unsigned short h = static_cast<unsigned short>(x[i >> 1] >> (16 * (i & 1)));
+        if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(h));
+        else return __uint_as_float(static_cast<uint32_t>(h) << 16);
+    }
+}
+
+struct SelectParams {
+    const void* logits;
+    const float* scores;
+    const uint8_t* finished;
+    float* scores_out;
+    int* parents_out;
+    int* tokens_out;
+    uint8_t* finished_out;
+    float2* tile_ml;  // [rows][tiles]: maximum and sum of exp(x - maximum)
+    u64* tile_top;    // [rows][tiles][n_out]: key_of(value) << 32 | ~index, descending; 0: none
+    long long ld;
+    int vocab, beams, tiles, n_out, eos;
+};
+
+// A row whose beam is not alive or is finished is not read.
+__device__ __forceinline__ bool row_counts(const SelectParams& p, int row) {
+    return isfinite(p.scores[row]) && !(p.finished && p.finished[row]);
+}
+
+// One CTA per tile of BS_THREADS * NV 16-byte vectors of a row, held in registers.  Rows may start anywhere: vectors
+// are cut on 16-byte boundaries of memory and the ragged ends are read element by element.
+template <typename T, int NV>
+__global__ void __launch_bounds__(BS_THREADS) beam_tile_kernel(const __grid_constant__ SelectParams p) {
+    constexpr int V = 16 / sizeof(T);
+    __shared__ Pool pool;
+    __shared__ u64 slots[BS_WARPS];
+    __shared__ float wm[BS_WARPS], wl[BS_WARPS];
+    izb::pdl_launch_dependents();
+    izb::pdl_wait();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int row = blockIdx.x / p.tiles, tile = blockIdx.x - row * p.tiles;
+    if (!row_counts(p, row)) return;
+    const T* base = static_cast<const T*>(p.logits) + static_cast<long long>(row) * p.ld;
+    const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
+    const int first = tile * (BS_THREADS * NV) + tid;
+    const uint32_t none = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;  // -inf
+
+    uint4 r[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const long long e0 = static_cast<long long>(first + i * BS_THREADS) * V - skew;
+        if (e0 >= 0 && e0 + V <= p.vocab) {
+            r[i] = __ldcs(reinterpret_cast<const uint4*>(base + e0));
+        } else {
+            uint32_t w[4] = {none, none, none, none};
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const long long e = e0 + k;
+                if (e >= 0 && e < p.vocab) {
+                    if constexpr (sizeof(T) == 4) w[k] = __float_as_uint(reinterpret_cast<const float*>(base)[e]);
+                    else
+                        w[k >> 1] = (w[k >> 1] & (0xFFFF0000u >> (16 * (k & 1)))) |
+                                    (static_cast<uint32_t>(reinterpret_cast<const unsigned short*>(base)[e]) << (16 * (k & 1)));
+                }
+            }
+            r[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    // only finite logits count: the others as -inf
+    auto at = [&](int i, int k) -> float {
+        const float x = element<T>(r[i], k);
+        return fabsf(x) < INFINITY ? x : -INFINITY;
+    };
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) mx = fmaxf(mx, at(i, k));
+    float top = mx;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    float sum = 0.f;
+    if (top > -INFINITY) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float part = 0.f;
+#pragma unroll
+            for (int k = 0; k < V; ++k) part += __expf(at(i, k) - top);
+            sum += part;
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if (lane == 0) {
+        wm[warp] = top;
+        wl[warp] = sum;
+    }
+    // every thread's largest value bounds the tile's n_out largest; ties are left to collect()
+    const u64 bound = block_bound(mx > -INFINITY ? static_cast<u64>(key_of(mx)) << 32 : 0ull, p.n_out, slots);
+    if (tid == 0) {
+        float m = -INFINITY, l = 0.f;
+        for (int w = 0; w < BS_WARPS; ++w) m = fmaxf(m, wm[w]);
+        for (int w = 0; w < BS_WARPS; ++w) l += wm[w] > -INFINITY ? wl[w] * __expf(wm[w] - m) : 0.f;
+        p.tile_ml[blockIdx.x] = make_float2(m, l);
+    }
+    const int n = collect(pool, bound, p.n_out, [&](u64 bk, uint32_t bi) {
+        const float floor_v = bk >> 32 ? value_of(static_cast<uint32_t>(bk >> 32)) : -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float x = at(i, k);
+                if (x >= floor_v && x > -INFINITY) {
+                    const uint32_t e = static_cast<uint32_t>(first + i * BS_THREADS) * V - skew + k;
+                    const u64 key = static_cast<u64>(key_of(x)) << 32;
+                    if (!before(bk, bi, key, e)) pool_add(pool, key, e);
+                }
+            }
+    });
+    u64* out = p.tile_top + static_cast<long long>(blockIdx.x) * p.n_out;
+    for (int i = tid; i < p.n_out; i += BS_THREADS) out[i] = i < n ? pool.key[i] | static_cast<uint32_t>(~pool.idx[i]) : 0ull;
+}
+
+// One CTA per group: log-sums of its beams, then the order of what the tiles kept.
+__global__ void __launch_bounds__(BS_THREADS) beam_join_kernel(const __grid_constant__ SelectParams p) {
+    __shared__ Pool pool;
+    __shared__ u64 slots[BS_WARPS];
+    __shared__ double offset[BS_MAX_BEAMS];  // score - lse
+    __shared__ uint8_t state[BS_MAX_BEAMS];  // 0: nothing, 1: its row, 2: finished
+    izb::pdl_launch_dependents();
+    izb::pdl_wait();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int group = blockIdx.x, row0 = group * p.beams;
+    for (int b = warp; b < p.beams; b += BS_WARPS) {
+        const float score = p.scores[row0 + b];
+        const bool alive = isfinite(score), done = p.finished && p.finished[row0 + b];
+        if (alive && !done) {
+            const float2* ml = p.tile_ml + static_cast<long long>(row0 + b) * p.tiles;
+            float m = -INFINITY;
+            for (int t = lane; t < p.tiles; t += 32) m = fmaxf(m, ml[t].x);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+            double s = 0.0;
+            for (int t = lane; t < p.tiles; t += 32) {
+                const float2 x = ml[t];
+                if (x.x > -INFINITY) s += static_cast<double>(x.y) * exp(static_cast<double>(x.x) - static_cast<double>(m));
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+            if (lane == 0) {
+                offset[b] = static_cast<double>(score) - (static_cast<double>(m) + log(s));
+                state[b] = m > -INFINITY ? 1 : 0;
+            }
+        } else if (lane == 0) {
+            offset[b] = static_cast<double>(score);
+            state[b] = alive && p.eos >= 0 ? 2 : 0;
+        }
+    }
+    __syncthreads();
+    // A list is a tile's sorted pairs; a finished beam is a list of its one candidate.
+    const int lists = p.beams * p.tiles;
+    auto list_at = [&](int list, int i, u64& key, uint32_t& idx) -> bool {
+        const int b = list / p.tiles, t = list - b * p.tiles;
+        if (state[b] == 2) {
+            key = key_of(offset[b]);
+            idx = static_cast<uint32_t>(b) * p.vocab + p.eos;
+            return t == 0 && i == 0;
+        }
+        if (state[b] == 0 || i >= p.n_out) return false;
+        const u64 x = p.tile_top[(static_cast<long long>(row0) * p.tiles + list) * p.n_out + i];
+        if (x == 0) return false;
+        key = key_of(static_cast<double>(value_of(static_cast<uint32_t>(x >> 32))) + offset[b]);
+        idx = static_cast<uint32_t>(b) * p.vocab + static_cast<uint32_t>(~x);
+        return true;
+    };
+    u64 mine = 0;
+    for (int l = tid; l < lists; l += BS_THREADS) {
+        u64 key;
+        uint32_t idx;
+        if (list_at(l, 0, key, idx) && key > mine) mine = key;
+    }
+    const u64 bound = block_bound(mine, p.n_out, slots);
+    const int n = collect(pool, bound, p.n_out, [&](u64 bk, uint32_t bi) {
+        for (int l = tid; l < lists; l += BS_THREADS) {
+            u64 key;
+            uint32_t idx;
+            for (int i = 0; list_at(l, i, key, idx) && !before(bk, bi, key, idx); ++i) pool_add(pool, key, idx);
+        }
+    });
+    for (int i = tid; i < p.n_out; i += BS_THREADS) {
+        float score = -INFINITY;
+        int parent = 0, token = p.eos >= 0 ? p.eos : 0;
+        bool done = false;
+        if (i < n) {
+            const uint32_t idx = pool.idx[i];
+            parent = static_cast<int>(idx / static_cast<uint32_t>(p.vocab));
+            token = static_cast<int>(idx - static_cast<uint32_t>(parent) * p.vocab);
+            score = static_cast<float>(value_of(pool.key[i]));
+            done = state[parent] == 2 || token == p.eos;
+        }
+        const long long o = static_cast<long long>(group) * p.n_out + i;
+        p.scores_out[o] = score;
+        p.parents_out[o] = parent;
+        p.tokens_out[o] = token;
+        if (p.finished_out) p.finished_out[o] = done ? 1 : 0;
+    }
+}
+
+int dtype_bytes(int dtype) { return dtype == IZB_F32 ? 4 : 2; }
+
+// 16-byte vectors per thread of a tile: eight keep enough loads in flight to stream; two when eight would leave SMs
+// without a tile, so that a few rows spread over the chip.
+struct SelectPlan {
+    int nv;
+    int64_t tiles;
+};
+SelectPlan select_plan(const izb_ctx* ctx, int dtype, int64_t rows, int64_t vocab) {
+    const int64_t v = 16 / dtype_bytes(dtype), vectors = (vocab + v - 1 + v - 1) / v;  // a row may start up to v - 1 elements into a vector
+    SelectPlan pl;
+    const int64_t wide = (vectors + BS_THREADS * 8 - 1) / (BS_THREADS * 8);
+    pl.nv = rows * wide >= (ctx && ctx->sm_count > 0 ? ctx->sm_count : 148) ? 8 : 2;
+    pl.tiles = (vectors + BS_THREADS * pl.nv - 1) / (BS_THREADS * pl.nv);
+    return pl;
+}
+size_t select_bytes(const SelectPlan& pl, int64_t rows, int n_out) {
+    return static_cast<size_t>(rows) * pl.tiles * (static_cast<size_t>(n_out) * sizeof(u64) + sizeof(float2));
+}
+
+template <typename T>
+cudaError_t launch_tiles(izb_ctx* ctx, cudaStream_t s, const SelectParams& p, int nv, unsigned grid) {
+    if (nv == 8) return izb::launch_chained(ctx, beam_tile_kernel<T, 8>, dim3(grid), dim3(BS_THREADS), 0, s, p);
+    return izb::launch_chained(ctx, beam_tile_kernel<T, 2>, dim3(grid), dim3(BS_THREADS), 0, s, p);
+}
+
+// ---- reordering of the paged caches --------------------------------------------------------------------------------
+// Child k continues beam parents[k].  The pages a parent has filled are shared from now on: their table entries are
+// copied.  Its last, partly filled page will be written by every child, so each child needs one of its own: the
+// first child of a parent keeps the parent's page, and the others take the pages of beams without a child, in
+// ascending order (there are exactly as many), and copy the rows held so far.  A page that is read is kept by
+// somebody and a page that is written belonged to nobody any more, so copies of one call never meet.
+
+constexpr int RO_MAX_BEAMS = 32;
+constexpr int RO_MAX_LAYERS = 64;
+constexpr int RO_THREADS = 256;
+
+struct LayerPtrs {
+    uint8_t* k;
+    uint8_t* v;
+    float* k_scales;
+    float* v_scales;
+};
+struct ReorderParams {
+    LayerPtrs layer[RO_MAX_LAYERS];
+    const int* table;
+    int* table_out;
+    const int* parents;
+    const int* lens;
+    int* status;
+    long long max_pages;
+    long long page_bytes, row_bytes;  // of the values
+    int page_scales, row_scales;      // floats; Int8: one per page whatever it holds
+    int beams, page_size, n_layers, splits;
+};
+
+// grid (layers * 2 * splits, groups * beams): CTA (0, child) also writes the child's table row
+__global__ void __launch_bounds__(RO_THREADS) kv_pages_reorder_kernel(const __grid_constant__ ReorderParams p) {
+    izb::pdl_launch_dependents();
+    izb::pdl_wait();
+    __shared__ int sh_parent, sh_src, sh_dst, sh_full, sh_held;
+    const int child = blockIdx.y % p.beams, row0 = blockIdx.y - child;
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        const unsigned all = 0xFFFFFFFFu;
+        const bool in = lane < p.beams;
+        int par = in ? p.parents[row0 + lane] : -1 - lane;  // lanes past the beams match nobody
+        const int len = p.lens[row0 + (in ? lane : 0)];
+        const int len0 = __shfl_sync(all, len, 0);
+        // beams of a group grow together, a parent is one of them and the pages they fill are in the table: else the
+        // group's rows are left as they are
+        const bool wrong = __any_sync(all, (in && (par < 0 || par >= p.beams)) || len != len0 || len0 < 0) ||
+                           static_cast<long long>(len0) > p.max_pages * p.page_size;
+        if (wrong) {
+            if (lane == 0 && child == 0 && blockIdx.x == 0) atomicExch(p.status, 9);
+            par = in ? lane : -1 - lane;
+        }
+        const int full = wrong ? 0 : len0 / p.page_size, held = wrong ? 0 : len0 - full * p.page_size;
+        const unsigned same = __match_any_sync(all, par);
+        const bool again = in && (same & ((1u << lane) - 1u)) != 0;  // not its parent's first child
+        const unsigned again_mask = __ballot_sync(all, again);
+        unsigned has_child = 0;
+        for (int b = 0; b < p.beams; ++b)
+            if (__any_sync(all, in && par == b)) has_child |= 1u << b;
+        if (lane == child) {
+            int from = par;
+            if (again) {  // the page of the i-th beam without a child, i: further children before this one
+                const unsigned left = ~has_child & (p.beams == 32 ? all : (1u << p.beams) - 1u);
+                from = static_cast<int>(__fns(left, 0, __popc(again_mask & ((1u << lane) - 1u)) + 1));
+            }
+            sh_parent = par;
+            sh_full = full;
+            sh_held = held;
+            sh_src = held ? p.table[(row0 + par) * p.max_pages + full] : 0;
+            sh_dst = held ? p.table[(row0 + from) * p.max_pages + full] : 0;
+        }
+    }
+    __syncthreads();
+    const int held = sh_held, full = sh_full;
+    if (blockIdx.x == 0) {
+        const int* mine = p.table + static_cast<long long>(blockIdx.y) * p.max_pages;
+        const int* theirs = p.table + (row0 + sh_parent) * p.max_pages;
+        int* out = p.table_out + static_cast<long long>(blockIdx.y) * p.max_pages;
+        for (long long c = threadIdx.x; c < p.max_pages; c += RO_THREADS)
+            out[c] = c < full ? theirs[c] : (c == full && held) ? sh_dst : mine[c];
+    }
+    if (!held || sh_src == sh_dst) return;
+    const int split = blockIdx.x % p.splits, which = (blockIdx.x / p.splits) & 1, layer = blockIdx.x / (2 * p.splits);
+    uint8_t* values = which ? p.layer[layer].v : p.layer[layer].k;
+    float* scales = which ? p.layer[layer].v_scales : p.layer[layer].k_scales;
+    const uint4* src = reinterpret_cast<const uint4*>(values + sh_src * p.page_bytes);
+    uint4* dst = reinterpret_cast<uint4*>(values + sh_dst * p.page_bytes);
+    const int n = static_cast<int>(held * p.row_bytes / 16);
+    constexpr int UN = 8;
+    for (int i0 = split * RO_THREADS * UN + threadIdx.x; i0 < n; i0 += p.splits * RO_THREADS * UN) {
+        uint4 w[UN];
+#pragma unroll
+        for (int j = 0; j < UN; ++j)
+            if (i0 + j * RO_THREADS < n) w[j] = __ldcs(src + i0 + j * RO_THREADS);
+#pragma unroll
+        for (int j = 0; j < UN; ++j)
+            if (i0 + j * RO_THREADS < n) __stcs(dst + i0 + j * RO_THREADS, w[j]);
+    }
+    if (scales && split == 0) {
+        const int m = p.row_scales ? held * p.row_scales : p.page_scales;
+        for (int i = threadIdx.x; i < m; i += RO_THREADS)
+            scales[static_cast<long long>(sh_dst) * p.page_scales + i] = scales[static_cast<long long>(sh_src) * p.page_scales + i];
+    }
+}
+
+// ---- walk back through the choices ---------------------------------------------------------------------------------
+// out[j, s] = tokens[s, b_s],  b_{s-1} = parents[s, b_s],  b at the last step = last[j].
+__global__ void __launch_bounds__(128)
+    beam_trace_kernel(const int* __restrict__ parents, const int* __restrict__ tokens, const int* __restrict__ last,
+                      int* __restrict__ out, int steps, int beams, int picks, long long groups, long long ld_out, int* status) {
+    izb::pdl_launch_dependents();
+    izb::pdl_wait();
+    const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (i >= groups * picks) return;
+    const long long group = i / picks;
+    int b = last[i];
+    for (int s = steps - 1; s >= 0; --s) {
+        if (b < 0 || b >= beams) {
+            atomicExch(status, 9);
+            for (; s >= 0; --s) out[i * ld_out + s] = -1;
+            return;
+        }
+        const long long at = (s * groups + group) * beams + b;
+        out[i * ld_out + s] = tokens[at];
+        b = parents[at];
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t izb_beam_select_workspace_bytes(const izb_ctx* ctx, int32_t dtype, int64_t groups, int32_t beams, int64_t vocab, int32_t n_out) {
+    if (groups <= 0 || beams <= 0 || beams > BS_MAX_BEAMS || vocab <= 0 || vocab > INT32_MAX / beams || n_out <= 0 || n_out > BS_MAX_OUT ||
+        groups > INT32_MAX / beams)
+        return 0;
+    return select_bytes(select_plan(ctx, dtype, groups * beams, vocab), groups * beams, n_out);
+}
+
+int32_t izb_beam_select(izb_ctx* ctx, izb_stream stream, const void* logits, int32_t dtype, int64_t groups, int32_t beams, int64_t vocab,
+                        int64_t ld, const float* scores, const uint8_t* finished, int32_t eos, int32_t n_out, float* scores_out,
+                        int32_t* parents_out, int32_t* tokens_out, uint8_t* finished_out, void* workspace, size_t workspace_bytes) {
+    if (!ctx || groups < 0 || beams <= 0 || vocab <= 0 || ld < vocab || n_out <= 0) return IZB_ERR_BAD_ARG;
+    if (dtype != IZB_F32 && dtype != IZB_BF16 && dtype != IZB_F16) return IZB_ERR_BAD_ARG;
+    if (eos >= vocab || (finished && eos < 0)) return IZB_ERR_BAD_ARG;  // a finished beam goes on with eos
+    if (groups == 0) return IZB_OK;
+    if (beams > BS_MAX_BEAMS || n_out > BS_MAX_OUT || vocab > INT32_MAX / beams || groups > INT32_MAX / beams) return IZB_ERR_UNSUPPORTED;
+    if (!logits || !scores || !scores_out || !parents_out || !tokens_out) return IZB_ERR_BAD_ARG;
+    if (!izb_aligned(logits, dtype_bytes(dtype)) || !izb_aligned(scores, 4) || !izb_aligned(scores_out, 4) || !izb_aligned(parents_out, 4) ||
+        !izb_aligned(tokens_out, 4))
+        return IZB_ERR_BAD_ARG;
+    const int64_t rows = groups * beams, outs = groups * n_out;
+    // a group's scores and marks are read before its results are written, so a call may update them in place: the whole
+    // array or none of it
+    const bool same_scores = scores == scores_out, same_marks = finished == finished_out;
+    if (same_scores ? n_out != beams : (scores_out < scores + rows && scores < scores_out + outs)) return IZB_ERR_BAD_ARG;
+    if (finished && finished_out && (same_marks ? n_out != beams : (finished_out < finished + rows && finished < finished_out + outs)))
+        return IZB_ERR_BAD_ARG;
+    const SelectPlan pl = select_plan(ctx, dtype, rows, vocab);
+    if (rows > INT32_MAX / pl.tiles) return IZB_ERR_UNSUPPORTED;
+    const size_t need = select_bytes(pl, rows, n_out);
+    if (!workspace || workspace_bytes < need || !izb_aligned(workspace, 8)) return IZB_ERR_BAD_ARG;
+    SelectParams p = {};
+    p.logits = logits;
+    p.scores = scores;
+    p.finished = finished;
+    p.scores_out = scores_out;
+    p.parents_out = parents_out;
+    p.tokens_out = tokens_out;
+    p.finished_out = finished_out;
+    p.tile_ml = static_cast<float2*>(workspace);
+    p.tile_top = reinterpret_cast<u64*>(p.tile_ml + rows * pl.tiles);
+    p.ld = ld;
+    p.vocab = static_cast<int>(vocab);
+    p.beams = beams;
+    p.tiles = static_cast<int>(pl.tiles);
+    p.n_out = n_out;
+    p.eos = eos;
+    izb::DeviceGuard guard(ctx->device);
+    if (!guard.ok) return IZB_ERR_LAUNCH;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const unsigned grid = static_cast<unsigned>(rows * pl.tiles);
+    if (dtype == IZB_F32) IZB_CUDA_TRY(launch_tiles<float>(ctx, s, p, pl.nv, grid));
+    else if (dtype == IZB_F16) IZB_CUDA_TRY(launch_tiles<__half>(ctx, s, p, pl.nv, grid));
+    else IZB_CUDA_TRY(launch_tiles<__nv_bfloat16>(ctx, s, p, pl.nv, grid));
+    IZB_CUDA_TRY(izb::launch_chained(ctx, beam_join_kernel, dim3(static_cast<unsigned>(groups)), dim3(BS_THREADS), 0, s, p));
+    ctx->launches.fetch_add(2, std::memory_order_relaxed);
+    return IZB_OK;
+}
+
+int32_t izb_kv_pages_reorder(izb_ctx* ctx, izb_stream stream, const izb_kv_pages* layers, int32_t n_layers, const int32_t* parents,
+                             int64_t groups, int32_t beams, const int32_t* seq_lens, int32_t* page_table_out) {
+    if (!ctx || groups < 0 || beams <= 0 || n_layers <= 0 || !layers) return IZB_ERR_BAD_ARG;
+    if (groups == 0) return IZB_OK;
+    if (beams > RO_MAX_BEAMS || n_layers > RO_MAX_LAYERS || groups > 65535 / beams) return IZB_ERR_UNSUPPORTED;
+    if (!parents || !seq_lens || !page_table_out) return IZB_ERR_BAD_ARG;
+    if (!izb_aligned(parents, 4) || !izb_aligned(seq_lens, 4) || !izb_aligned(page_table_out, 4)) return IZB_ERR_BAD_ARG;
+    const izb_kv_pages& a = layers[0];
+    if (!a.page_table || !izb_aligned(a.page_table, 4)) return IZB_ERR_BAD_ARG;
+    if (a.quantization < IZB_KV_NONE || a.quantization > IZB_KV_Q4_0 || a.page_size <= 0 || a.kv_heads <= 0 || a.max_pages_per_seq <= 0)
+        return IZB_ERR_BAD_ARG;
+    if (a.head_dim != 64 && a.head_dim != 128) return IZB_ERR_UNSUPPORTED;
+    if (a.page_size > INT32_MAX / a.kv_heads / a.head_dim / 2) return IZB_ERR_UNSUPPORTED;
+    // rows of the old table are read while rows of the new one are written
+    const int64_t entries = groups * beams * a.max_pages_per_seq;
+    if (page_table_out < a.page_table + entries && a.page_table < page_table_out + entries) return IZB_ERR_BAD_ARG;
+    ReorderParams p = {};
+    for (int i = 0; i < n_layers; ++i) {
+        const izb_kv_pages& l = layers[i];
+        if (l.page_table != a.page_table || l.quantization != a.quantization || l.page_size != a.page_size || l.kv_heads != a.kv_heads ||
+            l.head_dim != a.head_dim || l.max_pages_per_seq != a.max_pages_per_seq)
+            return IZB_ERR_BAD_ARG;
+        if (!l.k_values || !l.v_values || !izb_aligned(l.k_values, 16) || !izb_aligned(l.v_values, 16)) return IZB_ERR_BAD_ARG;
+        if (a.quantization != IZB_KV_NONE && (!l.k_scales || !l.v_scales || !izb_aligned(l.k_scales, 4) || !izb_aligned(l.v_scales, 4)))
+            return IZB_ERR_BAD_ARG;
+        p.layer[i] = {static_cast<uint8_t*>(l.k_values), static_cast<uint8_t*>(l.v_values),
+                      a.quantization == IZB_KV_NONE ? nullptr : l.k_scales, a.quantization == IZB_KV_NONE ? nullptr : l.v_scales};
+    }
+    p.table = a.page_table;
+    p.table_out = page_table_out;
+    p.parents = parents;
+    p.lens = seq_lens;
+    p.status = ctx->d_status + 6;
+    p.max_pages = a.max_pages_per_seq;
+    p.page_bytes = static_cast<long long>(izb_kv_page_bytes(a.quantization, a.page_size, a.kv_heads, a.head_dim));
+    p.row_bytes = p.page_bytes / a.page_size;
+    p.page_scales = static_cast<int>(izb_kv_page_scales(a.quantization, a.page_size, a.kv_heads, a.head_dim));
+    p.row_scales = a.quantization == IZB_KV_Q4_0 ? p.page_scales / a.page_size : 0;
+    p.beams = beams;
+    p.page_size = a.page_size;
+    p.n_layers = n_layers;
+    // 32 KB of a page per CTA and trip
+    const long long per = RO_THREADS * 8 * 16;
+    long long splits = (p.page_bytes + per - 1) / per;
+    p.splits = static_cast<int>(splits > 64 ? 64 : splits);
+    izb::DeviceGuard guard(ctx->device);
+    if (!guard.ok) return IZB_ERR_LAUNCH;
+    IZB_CUDA_TRY(izb::launch_chained(ctx, kv_pages_reorder_kernel, dim3(static_cast<unsigned>(n_layers * 2 * p.splits), static_cast<unsigned>(groups * beams)),
+                                     dim3(RO_THREADS), 0, static_cast<cudaStream_t>(stream), p));
+    ctx->launches.fetch_add(1, std::memory_order_relaxed);
+    return IZB_OK;
+}
+
+int32_t izb_beam_trace(izb_ctx* ctx, izb_stream stream, const int32_t* parents, const int32_t* tokens, int64_t steps, int64_t groups,
+                       int32_t beams, const int32_t* last, int32_t picks, int32_t* out, int64_t ld_out) {
+    if (!ctx || steps < 0 || groups < 0 || beams <= 0 || picks < 0 || ld_out < steps) return IZB_ERR_BAD_ARG;
+    if (steps == 0 || groups == 0 || picks == 0) return IZB_OK;
+    if (!parents || !tokens || !last || !out) return IZB_ERR_BAD_ARG;
+    if (!izb_aligned(parents, 4) || !izb_aligned(tokens, 4) || !izb_aligned(last, 4) || !izb_aligned(out, 4)) return IZB_ERR_BAD_ARG;
+    if (steps > INT32_MAX || groups > INT32_MAX / 128 || picks > INT32_MAX / groups) return IZB_ERR_UNSUPPORTED;
+    izb::DeviceGuard guard(ctx->device);
+    if (!guard.ok) return IZB_ERR_LAUNCH;
+    const unsigned grid = static_cast<unsigned>((groups * picks + 127) / 128);
+    IZB_CUDA_TRY(izb::launch_chained(ctx, beam_trace_kernel, dim3(grid), dim3(128), 0, static_cast<cudaStream_t>(stream), parents, tokens,
+                                     last, out, static_cast<int>(steps), beams, picks, static_cast<long long>(groups),
+                                     static_cast<long long>(ld_out), ctx->d_status + 6));
+    ctx->launches.fetch_add(1, std::memory_order_relaxed);
+    return IZB_OK;
+}
+
+}  // extern "C"

@@ -43,6 +43,26 @@ constexpr long long IZB_WAIT_LIMIT_CLOCKS = 2000000000LL;
 
 static inline bool izb_aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
+namespace izb {
+// Makes `device` current for the launches of an entry point and puts the caller's device back.
+struct DeviceGuard {
+    explicit DeviceGuard(int device) {
+        ok = cudaGetDevice(&prev) == cudaSuccess;
+        if (ok && prev != device) {
+            ok = changed = cudaSetDevice(device) == cudaSuccess;
+        }
+        if (!ok) (void)cudaGetLastError();
+    }
+    ~DeviceGuard() {
+        if (changed) (void)cudaSetDevice(prev);
+    }
+    DeviceGuard(const DeviceGuard&) = delete;
+    DeviceGuard& operator=(const DeviceGuard&) = delete;
+    int prev = 0;
+    bool ok = false, changed = false;
+};
+}  // namespace izb
+
 #ifdef __CUDACC__
 namespace izb {
 

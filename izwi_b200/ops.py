@@ -231,6 +231,66 @@ def sample_rows(logits: torch.Tensor, temperature: float, top_k: int, top_p: flo
     return idx.reshape(logits.shape[:-1])
 
 
+def _stream_of(t: torch.Tensor) -> C.c_void_p:
+    """The current stream of the tensor's device, whichever device is current."""
+    return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: int | None = None, finished: torch.Tensor | None = None,
+                eos: int = -1, out: tuple | None = None):
+    """The n_out best extensions of every group's beams (izb_beam_select).  logits [groups * beams, vocab] (or
+    [groups, beams, vocab]) bf16 / fp32 / fp16, scores [groups, beams] fp32, finished [groups, beams] uint8.
+    Returns (scores, parents, tokens, finished), each [groups, n_out]; `out` gives the four buffers (for
+    n_out == beams the scores and marks may be updated in place; the last one may be None)."""
+    if scores.dim() != 2 or scores.dtype != torch.float32 or not scores.is_contiguous():
+        raise ValueError("beam_select: scores must be contiguous fp32 [groups, beams]")
+    groups, beams = scores.shape
+    x = logits.reshape(-1, logits.shape[-1])
+    if x.dtype not in DTYPE or not x.is_cuda or x.stride(1) != 1 or x.shape[0] != groups * beams:
+        raise ValueError("beam_select: logits must be bf16 / fp32 / fp16 CUDA rows, one for each beam")
+    if finished is not None and (finished.shape != scores.shape or finished.dtype != torch.uint8 or not finished.is_contiguous()):
+        raise ValueError("beam_select: finished must be contiguous uint8 [groups, beams]")
+    dev = x.device
+    if scores.device != dev or (finished is not None and finished.device != dev):
+        raise ValueError("beam_select: tensors on different devices")
+    n = beams if n_out is None else int(n_out)
+    if out is None:
+        ints = torch.empty(2, groups, max(n, 0), device=dev, dtype=torch.int32)
+        out = (torch.empty(groups, max(n, 0), device=dev, dtype=torch.float32), ints[0], ints[1],
+               torch.empty(groups, max(n, 0), device=dev, dtype=torch.uint8))
+    else:
+        for t, d in zip(out, (torch.float32, torch.int32, torch.int32, torch.uint8)):
+            if t is not None and (t.shape != (groups, n) or t.dtype != d or t.device != dev or not t.is_contiguous()):
+                raise ValueError("beam_select: out must be contiguous [groups, n_out] fp32, int32, int32, uint8")
+    ctx = Context.get(dev.index)
+    lib = L.lib()
+    code, vocab = DTYPE[x.dtype], x.shape[1]
+    need = lib.izb_beam_select_workspace_bytes(ctx.handle, code, groups, beams, vocab, n)
+    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+    L.check(lib.izb_beam_select(ctx.handle, _stream_of(x), x.data_ptr(), code, groups, beams, vocab, x.stride(0) if groups * beams > 1 else vocab,
+                                scores.data_ptr(), None if finished is None else finished.data_ptr(), int(eos), n, out[0].data_ptr(),
+                                out[1].data_ptr(), out[2].data_ptr(), None if out[3] is None else out[3].data_ptr(), _ptr(ws), need),
+            "izb_beam_select")
+    return tuple(out)
+
+
+def beam_trace(parents: torch.Tensor, tokens: torch.Tensor, last: torch.Tensor) -> torch.Tensor:
+    """Token sequences [groups, picks, steps] of the beams `last` [groups, picks], walked back through the choices
+    parents / tokens [steps, groups, beams] (izb_beam_trace).  All int32, contiguous, on one device."""
+    if parents.dim() != 3 or parents.shape != tokens.shape or last.dim() != 2 or last.shape[0] != parents.shape[1]:
+        raise ValueError("beam_trace: parents and tokens must be [steps, groups, beams], last [groups, picks]")
+    for t in (parents, tokens, last):
+        if t.dtype != torch.int32 or not t.is_contiguous() or not t.is_cuda or t.device != parents.device:
+            raise ValueError("beam_trace: contiguous int32 CUDA tensors of one device")
+    steps, groups, beams = parents.shape
+    picks = last.shape[1]
+    out = torch.empty(groups, picks, steps, device=parents.device, dtype=torch.int32)
+    ctx = Context.get(parents.device.index)
+    L.check(L.lib().izb_beam_trace(ctx.handle, _stream_of(parents), parents.data_ptr(), tokens.data_ptr(), steps, groups, beams,
+                                   last.data_ptr(), picks, out.data_ptr(), steps), "izb_beam_trace")
+    return out
+
+
 def rope_pair_(q: torch.Tensor, k: torch.Tensor, cos_half: torch.Tensor, sin_half: torch.Tensor) -> None:
     """`apply_rotary_emb` on q and k (qwen3/core.rs:2402-2415), in place.  q [tokens, q_heads, d],
     k [tokens, k_heads, d], tables [tokens, d / 2]; all bf16."""

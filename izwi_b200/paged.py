@@ -9,7 +9,7 @@ import ctypes as C
 import torch
 
 from . import _lib as L
-from .ops import Context, _ptr, _stream
+from .ops import Context, _ptr, _stream, _stream_of
 
 DEFAULT_KV_PAGE_SIZE = 64                     # paged.rs:10
 QUANT = {"none": 0, "int8": 1, "q4_0": 2}
@@ -47,9 +47,42 @@ class PagedKvCache:
         self.page_table = torch.arange(n_pages, device=device, dtype=torch.int32).reshape(batch, self.max_pages).contiguous()
         self.seq_lens = torch.zeros(batch, device=device, dtype=torch.int32)
         self.max_tokens = self.max_pages * page_size
-        self._desc = L.KvPages(self.k_values.data_ptr(), self.v_values.data_ptr(), self.k_scales.data_ptr() if nscales else None,
-                               self.v_scales.data_ptr() if nscales else None, self.page_table.data_ptr(), q, page_size, kv_heads,
-                               head_dim, self.max_pages)
+        self._describe()
+
+    def _describe(self) -> None:
+        q = QUANT[self.quantization]
+        self._desc = L.KvPages(self.k_values.data_ptr(), self.v_values.data_ptr(), self.k_scales.data_ptr() if q else None,
+                               self.v_scales.data_ptr() if q else None, self.page_table.data_ptr(), q, self.page_size, self.kv_heads,
+                               self.head_dim, self.max_pages)
+
+    @classmethod
+    def view(cls, k_values: torch.Tensor, v_values: torch.Tensor, k_scales: torch.Tensor | None, v_scales: torch.Tensor | None,
+             page_table: torch.Tensor, seq_lens: torch.Tensor, kv_heads: int, head_dim: int, quantization: str = "none",
+             page_size: int = DEFAULT_KV_PAGE_SIZE) -> "PagedKvCache":
+        """A cache over buffers that the caller owns: pools of whole pages (any type, contiguous), their fp32 scales, the
+        page table [sequences, max_pages] and the lengths [sequences], both int32.  Several layers may name one table."""
+        if page_size <= 0:
+            raise ValueError("KV page size must be greater than zero")
+        if page_table.dim() != 2 or page_table.dtype != torch.int32 or seq_lens.dtype != torch.int32 or seq_lens.shape != page_table.shape[:1]:
+            raise ValueError("a page table is int32 [sequences, max_pages], lengths are int32 [sequences]")
+        q, lib = QUANT[quantization], L.lib()
+        nbytes, nscales = lib.izb_kv_page_bytes(q, page_size, kv_heads, head_dim), lib.izb_kv_page_scales(q, page_size, kv_heads, head_dim)
+        tensors = [k_values, v_values, page_table, seq_lens] + ([k_scales, v_scales] if nscales else [])
+        if any(t is None or not t.is_cuda or not t.is_contiguous() or t.device != page_table.device for t in tensors):
+            raise ValueError("page buffers must be contiguous CUDA tensors of one device")
+        pool = k_values.numel() * k_values.element_size()
+        if nbytes == 0 or pool % nbytes or v_values.numel() * v_values.element_size() != pool:
+            raise ValueError("page pools must hold whole pages, as many for values as for keys")
+        if nscales and any(t.dtype != torch.float32 or t.numel() != pool // nbytes * nscales for t in (k_scales, v_scales)):
+            raise ValueError("page scales must be fp32, as many as the pool's pages need")
+        self = cls.__new__(cls)
+        self.batch, self.max_pages = page_table.shape
+        self.kv_heads, self.head_dim, self.page_size, self.quantization = kv_heads, head_dim, page_size, quantization
+        self.k_values, self.v_values, self.k_scales, self.v_scales = k_values, v_values, k_scales, v_scales
+        self.page_table, self.seq_lens = page_table, seq_lens
+        self.max_tokens = self.max_pages * page_size
+        self._describe()
+        return self
 
     def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
         """k, v [batch, n_new, kv_heads, head_dim] bf16 (the reference's `[batch, seq, heads, dim]`)."""
@@ -86,3 +119,89 @@ class PagedKvCache:
                                                        float(d ** -0.5 if scale is None else scale), _ptr(ws), need),
                 "izb_paged_decode_gqa_attention")
         return out
+
+
+def shared_prefix_attention(q: torch.Tensor, prefix: PagedKvCache, suffix: PagedKvCache | None, scale: float | None = None,
+                            max_prefix_len: int | None = None, max_seq_len: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Single-token attention of sequences that share a prompt (izb_shared_prefix_decode_gqa_attention): q
+    [groups * n, heads, head_dim] bf16, `prefix` one sequence per group, `suffix` one per row of q, or None.
+    Sequence i attends to the whole of prefix i // n and then to its own suffix.  The two bounds (default: what the
+    tables hold) only size the split over the device."""
+    b, h, d = q.shape
+    if q.dtype != torch.bfloat16 or not q.is_cuda or q.stride(2) != 1 or q.stride(1) != d:
+        raise ValueError("shared_prefix_attention: q must be bf16 [sequences, heads, head_dim] with dense heads")
+    groups = prefix.batch
+    if groups == 0 or b % groups != 0 or d != prefix.head_dim or h % prefix.kv_heads != 0:
+        raise ValueError(f"shared_prefix_attention: q {tuple(q.shape)} does not fit {groups} prefixes of {prefix.kv_heads} x {prefix.head_dim}")
+    if suffix is not None and (suffix.batch != b or suffix.kv_heads != prefix.kv_heads or suffix.head_dim != d):
+        raise ValueError("shared_prefix_attention: the suffix must hold one sequence per query, with the prefix's heads")
+    if prefix.page_table.device != q.device or (suffix is not None and suffix.page_table.device != q.device):
+        raise ValueError("shared_prefix_attention: tensors on different devices")
+    if out is None:
+        out = torch.empty(b, h, d, device=q.device, dtype=torch.bfloat16)
+    elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != q.device or out.stride(2) != 1 or out.stride(1) != d:
+        raise ValueError("shared_prefix_attention: out must be like q")
+    if b == 0:
+        return out
+    most_p = prefix.max_tokens if max_prefix_len is None else int(max_prefix_len)
+    most_s = 0 if suffix is None else suffix.max_tokens if max_seq_len is None else int(max_seq_len)
+    ctx, lib = Context.get(q.device.index), L.lib()
+    need = lib.izb_shared_prefix_decode_gqa_attention_workspace_bytes(ctx.handle, groups, b // groups, h, prefix.kv_heads, d, most_p, most_s)
+    ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
+    L.check(lib.izb_shared_prefix_decode_gqa_attention(
+        ctx.handle, _stream_of(q), q.data_ptr(), C.byref(prefix._desc), prefix.seq_lens.data_ptr(),
+        None if suffix is None else C.byref(suffix._desc), None if suffix is None else suffix.seq_lens.data_ptr(), out.data_ptr(), groups,
+        b // groups, h, most_p, most_s, q.stride(0) if b > 1 else h * d, out.stride(0) if b > 1 else h * d, float(d ** -0.5 if scale is None else scale), _ptr(ws), need),
+        "izb_shared_prefix_decode_gqa_attention")
+    return out
+
+
+class PagedLayers:
+    """The caches of a model's layers for the beams of a search: they share one page table, so that a step's choice
+    reorders all of them by one launch (izb_kv_pages_reorder)."""
+
+    def __init__(self, caches: list[PagedKvCache]):
+        if not caches:
+            raise ValueError("PagedLayers needs at least one cache")
+        a = caches[0]
+        for c in caches:
+            if c.page_table.data_ptr() != a.page_table.data_ptr() or c.page_table.shape != a.page_table.shape:
+                raise ValueError("the layers of a PagedLayers must share one page table")
+        self.caches, self.batch = caches, a.batch
+        self._array = (L.KvPages * len(caches))(*(c._desc for c in caches))
+
+    @classmethod
+    def allocate(cls, n_layers: int, sequences: int, kv_heads: int, head_dim: int, max_tokens: int, device, quantization: str = "none",
+                 page_size: int = DEFAULT_KV_PAGE_SIZE) -> "PagedLayers":
+        """Empty caches of n_layers layers for `sequences` beams of up to max_tokens tokens each."""
+        caches = [PagedKvCache(sequences, kv_heads, head_dim, max_tokens, device, quantization, page_size) for _ in range(n_layers)]
+        for c in caches[1:]:
+            c.page_table = caches[0].page_table
+            c._describe()
+        return cls(caches)
+
+    def reorder(self, parents: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+        """Page table under which sequence g * beams + k continues sequence g * beams + parents[g, k]; pages that several
+        beams would go on writing are copied.  parents [groups, beams] int32.  The caches go on using the old table until
+        `use` is called with the new one."""
+        table = self.caches[0].page_table
+        if parents.dim() != 2 or parents.dtype != torch.int32 or not parents.is_contiguous() or parents.numel() != self.batch \
+                or parents.device != table.device:
+            raise ValueError(f"reorder: parents must be contiguous int32 [groups, beams] for {self.batch} sequences")
+        if out is None:
+            out = torch.empty_like(table)
+        elif out.shape != table.shape or out.dtype != torch.int32 or not out.is_contiguous() or out.device != table.device:
+            raise ValueError("reorder: out must be like the page table")
+        ctx = Context.get(table.device.index)
+        L.check(L.lib().izb_kv_pages_reorder(ctx.handle, _stream_of(table), self._array, len(self.caches), parents.data_ptr(), parents.shape[0],
+                                             parents.shape[1], self.caches[0].seq_lens.data_ptr(), out.data_ptr()), "izb_kv_pages_reorder")
+        return out
+
+    def use(self, table: torch.Tensor) -> None:
+        """Makes `table` the page table of all layers."""
+        if table.shape != self.caches[0].page_table.shape or table.dtype != torch.int32 or not table.is_contiguous() \
+                or table.device != self.caches[0].page_table.device:
+            raise ValueError("use: the new page table must be like the old one")
+        for i, c in enumerate(self.caches):
+            c.page_table = table
+            c._desc.page_table = self._array[i].page_table = table.data_ptr()

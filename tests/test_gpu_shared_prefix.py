@@ -1,0 +1,255 @@
+"""Attention of sequences that share a prompt (izb_shared_prefix_decode_gqa_attention) against softmax attention in 64 bits
+over the stored values, token by token through the page tables.
+
+Tolerance.  The kernel's result differs from the exact one by the rounding of the output (at most 2^-8 of it, half a
+bf16 step), the rounding of the weights for the product with v (2^-8 of each term, so 2^-8 of A = sum p |v| / sum p), and
+fp32 arithmetic: scores of D products (D 2^-24 of B = scale sum |q| |k|, which moves a weight by that much, both in the
+numerator and in the sum) and accumulation over the tokens (T 2^-24 of A).  Q4_0 scales that are no bf16 numbers: a
+stored value is the product of code and scale rounded to bf16; the kernel may land on the neighbour when the product is
+within 2^-17 of a tie, so it is held to the unrounded product, from which both lie at most 2^-8 (1 + 2^-8) away: weights
+move by that times 2 B, values by that."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+HALF = 2.0 ** -8
+
+
+class Pool:
+    """A paged cache with random contents; every slot past a sequence's end holds NaN, the table is shuffled."""
+
+    def __init__(self, rng, cuda, lens, kvh, d, page, quant, spare_pages=1, bf16_scales=True):
+        from izwi_b200 import paged
+        self.lens, self.page, self.kvh, self.d, self.quant = lens, page, kvh, d, quant
+        rows, per = len(lens), max(1, -(-max(lens) // page)) + spare_pages
+        n = rows * per
+        table = rng.permutation(n).astype(np.int32).reshape(rows, per)
+        self.exact = []  # per sequence: (k, v), [len, kvh, d] float64
+        used = np.zeros((n, page), bool)
+        for r, m in enumerate(lens):
+            for t in range(m):
+                used[table[r, t // page], t % page] = True
+        bufs, scales, values = [], [], []
+        for _ in "kv":
+            if quant == "none":
+                x = torch.from_numpy(rng.normal(0, 1, (n, page, kvh, d)).astype(np.float32)).to(torch.bfloat16)
+                x[torch.from_numpy(~used)] = float("nan")
+                values.append(x.double().numpy())
+                bufs.append(x.reshape(-1).to(cuda))
+                scales.append(None)
+            elif quant == "int8":
+                code = rng.integers(1, 256, (n, page, kvh, d)).astype(np.uint8)
+                sc = rng.uniform(0.005, 0.02, n).astype(np.float32)
+                sc[~used.any(1)] = np.nan
+                sb = torch.from_numpy(sc).to(torch.bfloat16).double().numpy()
+                values.append(torch.from_numpy((code.astype(np.float64) - 128) * sb[:, None, None, None]).float().to(torch.bfloat16).double().numpy())
+                bufs.append(torch.from_numpy(code.reshape(-1)).to(cuda))
+                scales.append(torch.from_numpy(sc).to(cuda))
+            else:
+                code = rng.integers(1, 16, (n, page, kvh, d)).astype(np.uint8)
+                sc = rng.uniform(0.05, 0.3, (n, page, kvh, d // 32)).astype(np.float32)
+                if bf16_scales:
+                    sc = torch.from_numpy(sc).to(torch.bfloat16).float().numpy()
+                sc[~used] = np.nan
+                x = (code.astype(np.float64) - 8) * np.repeat(sc.astype(np.float64), 32, axis=-1)
+                values.append(torch.from_numpy(x).float().to(torch.bfloat16).double().numpy() if bf16_scales else x)
+                flat = code.reshape(-1, 2)
+                bufs.append(torch.from_numpy((flat[:, 0] | (flat[:, 1] << 4)).astype(np.uint8)).to(cuda))
+                scales.append(torch.from_numpy(sc.reshape(-1)).to(cuda))
+        for r, m in enumerate(lens):
+            t = np.arange(m)
+            self.exact.append(tuple(v[table[r, t // page], t % page] for v in values))
+        self.cache = paged.PagedKvCache.view(bufs[0], bufs[1], scales[0], scales[1], torch.from_numpy(table).to(cuda),
+                                             torch.tensor(lens, dtype=torch.int32, device=cuda), kvh, d, quant, page)
+
+
+def check(rng, cuda, seqs, heads, prefix, suffix, scale=None, value_off=0.0, **kw):
+    """One call against the definition; returns the output."""
+    from izwi_b200 import ops, paged
+    d, kvh = prefix.d, prefix.kvh
+    b = len(prefix.lens) * seqs
+    q = torch.from_numpy(rng.normal(0, 2, (b, heads, d)).astype(np.float32)).to(torch.bfloat16)
+    got = paged.shared_prefix_attention(q.to(cuda), prefix.cache, None if suffix is None else suffix.cache, scale, **kw)
+    ops.Context.get(0).check()
+    got = got.double().cpu().numpy()
+    qd, g = q.double().numpy(), heads // kvh
+    sc = d ** -0.5 if scale is None else scale
+    for i in range(b):
+        k, v = prefix.exact[i // seqs]
+        if suffix is not None:
+            k, v = np.concatenate([k, suffix.exact[i][0]]), np.concatenate([v, suffix.exact[i][1]])
+        if len(k) == 0:
+            assert (got[i] == 0).all(), "a sequence without any token gives zeros"
+            continue
+        kr, vr = np.repeat(k, g, axis=1), np.repeat(v, g, axis=1)             # [T, heads, d]
+        s = np.einsum("hd,thd->ht", qd[i], kr) * sc
+        p = np.exp(s - s.max(1, keepdims=True))
+        p /= p.sum(1, keepdims=True)
+        want = np.einsum("ht,thd->hd", p, vr)
+        a = np.einsum("ht,thd->hd", p, np.abs(vr))
+        mag = abs(sc) * np.einsum("hd,thd->ht", np.abs(qd[i]), np.abs(kr)).max(1, keepdims=True)
+        moved = np.expm1(2 * mag * (value_off + (d + 4) * 2.0 ** -24))
+        tol = HALF * np.abs(want) + a * (HALF + len(k) * 2.0 ** -24 + 2.0 ** -20 + moved + value_off) * (1 + HALF)
+        err = np.abs(got[i] - want)
+        assert (err <= tol).all(), f"sequence {i}: {(err / tol).max():.2f} of the tolerance"
+    return got
+
+
+@pytest.mark.parametrize("quant", ["none", "int8", "q4_0"])
+@pytest.mark.parametrize("seqs,heads,kvh,d,page,plens,slens", [
+    (1, 1, 1, 64, 64, [1], [1]),                       # one row, one token each
+    (1, 8, 8, 128, 64, [0], [3]),                      # no prefix
+    (4, 16, 8, 128, 64, [100], [5, 5, 5, 5]),
+    (5, 4, 4, 64, 5, [63, 64], [0, 1, 2, 64, 65, 7, 0, 3, 130, 4]),   # ragged, pages that end inside a tile
+    (4, 16, 4, 128, 16, [65, 0, 129], [0, 0, 0, 0, 1, 0, 2, 0, 9, 9, 9, 9]),  # some sequences with nothing at all
+    (3, 32, 2, 64, 7, [200], [33, 1, 0]),              # 48 rows, sixteen query heads per KV head
+    (17, 8, 2, 128, 64, [300], [6] * 17),              # 68 rows: the wide block, partly filled
+    (33, 8, 2, 64, 128, [257], [1] * 33),              # 132 rows: a second row block of four
+    (2, 2, 1, 128, 1, [70], [3, 4]),                   # pages of one token
+])
+def test_against_the_definition(cuda, quant, seqs, heads, kvh, d, page, plens, slens):
+    rng = np.random.default_rng(seqs * 100 + heads + sum(plens))
+    prefix = Pool(rng, cuda, plens, kvh, d, page, quant)
+    suffix = Pool(rng, cuda, slens, kvh, d, page, quant)
+    check(rng, cuda, seqs, heads, prefix, suffix)
+
+
+@pytest.mark.parametrize("quant", ["none", "int8", "q4_0"])
+@pytest.mark.parametrize("seqs,heads,kvh,d,plens", [(5, 20, 20, 64, [1500, 1400]), (8, 8, 8, 128, [5000]), (20, 4, 2, 64, [2500])])
+def test_prefix_alone_and_many_chunks(cuda, quant, seqs, heads, kvh, d, plens):
+    rng = np.random.default_rng(seqs + heads)
+    check(rng, cuda, seqs, heads, Pool(rng, cuda, plens, kvh, d, 64, quant), None)
+
+
+@pytest.mark.parametrize("pq,sq", [("int8", "none"), ("none", "q4_0"), ("q4_0", "int8")])
+def test_prefix_and_suffix_stored_differently(cuda, pq, sq):
+    rng = np.random.default_rng(3)
+    prefix, suffix = Pool(rng, cuda, [333, 90], 4, 128, 64, pq), Pool(rng, cuda, [20, 0, 70, 1, 64, 65], 4, 128, 16, sq)
+    check(rng, cuda, 3, 8, prefix, suffix)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_q4_0_scales_of_full_precision(cuda, d):
+    rng = np.random.default_rng(8)
+    prefix = Pool(rng, cuda, [150], 2, d, 64, "q4_0", bf16_scales=False)
+    suffix = Pool(rng, cuda, [9, 70], 2, d, 64, "q4_0", bf16_scales=False)
+    check(rng, cuda, 2, 4, prefix, suffix, value_off=HALF * (1 + HALF))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.05, 0.5])
+def test_scales_of_any_sign(cuda, scale):
+    rng = np.random.default_rng(9)
+    check(rng, cuda, 2, 4, Pool(rng, cuda, [130], 2, 64, 64, "none"), Pool(rng, cuda, [3, 67], 2, 64, 64, "none"), scale=scale)
+
+
+def test_one_row_does_not_depend_on_the_others(cuda):
+    """The same sequence alone, with others in its group, and with bounds given: within two roundings of each other."""
+    from izwi_b200 import paged
+    rng = np.random.default_rng(5)
+    prefix, suffix = Pool(rng, cuda, [700], 2, 128, 64, "none"), Pool(rng, cuda, [40] * 6, 2, 128, 64, "none")
+    q = torch.from_numpy(rng.normal(0, 1, (6, 8, 128)).astype(np.float32)).to(cuda).to(torch.bfloat16)
+    both = paged.shared_prefix_attention(q, prefix.cache, suffix.cache)
+    tight = paged.shared_prefix_attention(q, prefix.cache, suffix.cache, max_prefix_len=700, max_seq_len=40)
+    one = paged.PagedKvCache.view(suffix.cache.k_values, suffix.cache.v_values, None, None, suffix.cache.page_table[2:3].contiguous(),
+                                  suffix.cache.seq_lens[2:3].contiguous(), 2, 128, "none", 64)
+    alone = paged.shared_prefix_attention(q[2:3], prefix.cache, one)
+    for other in (tight[2], alone[0]):
+        diff = (both[2].double() - other.double()).abs()
+        assert (diff <= 4 * HALF * both[2].double().abs() + 2 * HALF * 0.2).all()
+
+
+def test_lengths_are_cut_to_the_bounds(cuda):
+    """A length on the device beyond the bound counts up to the bound; a negative one counts nothing."""
+    from izwi_b200 import ops, paged
+    rng = np.random.default_rng(6)
+    prefix, suffix = Pool(rng, cuda, [100], 2, 64, 64, "none"), Pool(rng, cuda, [30, 30], 2, 64, 64, "none")
+    q = torch.from_numpy(rng.normal(0, 1, (2, 4, 64)).astype(np.float32)).to(cuda).to(torch.bfloat16)
+    want = paged.shared_prefix_attention(q, prefix.cache, None, max_prefix_len=100)
+    prefix.cache.seq_lens.fill_(2 ** 30)
+    suffix.cache.seq_lens.fill_(-7)
+    got = paged.shared_prefix_attention(q, prefix.cache, suffix.cache, max_prefix_len=100)
+    ops.Context.get(0).check()
+    diff = (got.double() - want.double()).abs()
+    assert (diff <= 2 * HALF * want.double().abs() + 2 * HALF * 0.5).all()
+
+
+def test_non_finite_queries_stay_in_their_rows(cuda):
+    from izwi_b200 import paged
+    rng = np.random.default_rng(7)
+    prefix = Pool(rng, cuda, [90], 2, 64, 64, "none")
+    q = torch.from_numpy(rng.normal(0, 1, (3, 4, 64)).astype(np.float32)).to(cuda).to(torch.bfloat16)
+    clean = paged.shared_prefix_attention(q, prefix.cache, None)
+    q[1, 2, 5] = float("nan")
+    got = paged.shared_prefix_attention(q, prefix.cache, None)
+    assert got[1, 2].isnan().all()
+    got[1, 2] = clean[1, 2]
+    assert torch.equal(got, clean)
+
+
+def test_strided_queries_streams_and_graph_replay(cuda):
+    """Rows of q and out apart; a side stream; a captured call replayed with other lengths and queries."""
+    from izwi_b200 import paged
+    rng = np.random.default_rng(11)
+    prefix, suffix = Pool(rng, cuda, [400, 130], 4, 128, 64, "int8"), Pool(rng, cuda, [9, 64, 0, 70], 4, 128, 64, "none")
+    wide = torch.from_numpy(rng.normal(0, 1, (4, 3, 8, 128)).astype(np.float32)).to(cuda).to(torch.bfloat16)
+    q = wide[:, 1]
+    want = paged.shared_prefix_attention(q.contiguous(), prefix.cache, suffix.cache)
+    room = torch.full((4, 2, 8, 128), 7.0, device=cuda, dtype=torch.bfloat16)
+    paged.shared_prefix_attention(q, prefix.cache, suffix.cache, out=room[:, 0])
+    assert torch.equal(room[:, 0], want) and (room[:, 1] == 7.0).all()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = paged.shared_prefix_attention(q, prefix.cache, suffix.cache)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(again, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = paged.shared_prefix_attention(q, prefix.cache, suffix.cache)
+    graph.replay()
+    assert torch.equal(out, want)
+    prefix.cache.seq_lens.copy_(torch.tensor([17, 128]))
+    suffix.cache.seq_lens.copy_(torch.tensor([1, 2, 0, 64]))
+    wide.mul_(0.5)
+    graph.replay()
+    assert torch.equal(out, paged.shared_prefix_attention(q, prefix.cache, suffix.cache)) and not torch.equal(out, want)
+    # two calls under way on two streams with workspaces of their own
+    outs = [paged.shared_prefix_attention(q, prefix.cache, suffix.cache) for _ in range(1)]
+    with torch.cuda.stream(side):
+        outs += [paged.shared_prefix_attention(q, prefix.cache, suffix.cache) for _ in range(3)]
+    outs += [paged.shared_prefix_attention(q, prefix.cache, suffix.cache) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, out) for o in outs)
+
+
+def test_empty_calls(cuda):
+    from izwi_b200 import paged
+    rng = np.random.default_rng(1)
+    prefix = Pool(rng, cuda, [10], 2, 64, 64, "none")
+    q = torch.zeros(0, 4, 64, device=cuda, dtype=torch.bfloat16)
+    assert paged.shared_prefix_attention(q, prefix.cache, None).shape == (0, 4, 64)
+    q = torch.ones(2, 4, 64, device=cuda, dtype=torch.bfloat16)
+    assert (paged.shared_prefix_attention(q, prefix.cache, None, max_prefix_len=0) == 0).all()
+
+
+def test_agrees_with_paged_attention_over_copies_of_the_prompt(cuda):
+    """The same continuations with the prompt copied into each sequence's pages (the entry point that was there)."""
+    from izwi_b200 import paged
+    rng = np.random.default_rng(12)
+    n, kvh, d, p, s = 3, 4, 128, 150, 20
+    k = torch.from_numpy(rng.normal(0, 1, (n, p + s, kvh, d)).astype(np.float32)).to(cuda).to(torch.bfloat16)
+    v = torch.from_numpy(rng.normal(0, 1, (n, p + s, kvh, d)).astype(np.float32)).to(cuda).to(torch.bfloat16)
+    k[:, :p], v[:, :p] = k[:1, :p], v[:1, :p]
+    whole = paged.PagedKvCache(n, kvh, d, p + s, cuda)
+    whole.append(k, v)
+    prefix, suffix = paged.PagedKvCache(1, kvh, d, p, cuda), paged.PagedKvCache(n, kvh, d, s, cuda)
+    prefix.append(k[:1, :p].contiguous(), v[:1, :p].contiguous())
+    suffix.append(k[:, p:].contiguous(), v[:, p:].contiguous())
+    q = torch.from_numpy(rng.normal(0, 1, (n, 8, d)).astype(np.float32)).to(cuda).to(torch.bfloat16)
+    a, b = whole.decode_attention(q).double(), paged.shared_prefix_attention(q, prefix, suffix).double()
+    # each within half a step of the output and 2^-8 A of the exact result; A <= max |v|, here bounded by 1
+    assert ((a - b).abs() <= 2 * HALF * a.abs() + 2 * HALF * 1.0).all()
+    assert math.isfinite(float(a.sum()))
