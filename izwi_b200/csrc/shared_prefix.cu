@@ -8,19 +8,20 @@
 // once and its 16-bit fragments are used by S * G rows on the tensor cores.
 //
 // Work: an item is (group, KV head, block of query rows, chunk of prefix tokens) or (sequence, KV head, chunk of its
-// own tokens); all items go out in one launch, one CTA each.  A CTA walks its chunk in tiles of 64 tokens with a
-// running maximum and sum per row and leaves (max, sum, weighted values) for a second launch that joins the chunks
+// own tokens); all items go out in one launch, one CTA each.  A CTA walks its chunk in tiles with a running maximum
+// and sum per row and leaves (max, sum, weighted values) for a second launch that joins the chunks
 // of every (sequence, head).  fp32 for scores, maxima, sums and accumulators; p is rounded to bf16 for the product
 // with v (half a step: 2^-9 relative, independent per token, which is what the bf16 output itself carries).
 #include <climits>
+#include <cmath>
 
 #include "izb_common.cuh"
 
 namespace {
 
-constexpr int SP_THREADS = 128;
-constexpr int SP_TILE = 64;          // tokens per tile
-constexpr int SP_MAX_CHUNK = 2048;   // tokens per item: bounds the shared table of token places
+constexpr int SP_THREADS = 256;      // four computing warps, four that copy
+constexpr int SP_TILE = 128;         // chunks are multiples of this, and so of every tile size
+constexpr int SP_MAX_CHUNK = 768;    // tokens per item: with their table of places two CTAs still share an SM
 constexpr int SP_MAX_G = 16;         // query heads per KV head: the rows of one own-pages item
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -46,20 +47,19 @@ struct Params {
     long long ld_q;
     int seqs, heads, kv_heads, g;  // sequences per group, query heads per KV head
     int row_blocks, prefix_items;
-    float scale_log2;
+    int* status;
+    uint32_t q_sign;   // flips q where the scale is negative, so that the largest product is the largest score
+    float scale_log2;  // |scale| / ln 2
+    float margin;      // 8 / scale_log2: a growth of 2^8 in weight, in units of the products
 };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool fill) {
-    const int n = fill ? 16 : 0;
+// `n` of the 16 (4) bytes come from src, the rest is zero
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int n) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool fill) {
-    const int n = fill ? 4 : 0;
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, int n) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
@@ -74,11 +74,6 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t r;
     asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
@@ -91,12 +86,12 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // Two Int8 codes in the low bytes of the halves of x (code = byte - 128) -> bf16x2.  128 + (byte & 127) is the bf16
-// 0x4300 | low bits; what is left is -256 for bytes below 128 and -128 above: every step is exact.
+// 0x4300 | low bits; what is left to add is -256 for bytes below 128 and -128 above: every step is exact.
 __device__ __forceinline__ uint32_t int8_pair(uint32_t x) {
-    return hsub2((x & 0x007F007Fu) | 0x43004300u, (~x & 0x00800080u) | 0x43004300u);
+    return hfma2((x & 0x007F007Fu) | 0x43004300u, 0x3F803F80u, (~x & 0x00800080u) | 0xC300C300u);
 }
 // Two 4-bit codes in the low nibbles of the halves (code = nibble - 8) -> bf16x2, exact.
-__device__ __forceinline__ uint32_t q4_pair(uint32_t x) { return hsub2((x & 0x000F000Fu) | 0x43004300u, 0x43084308u); }
+__device__ __forceinline__ uint32_t q4_pair(uint32_t x) { return hfma2((x & 0x000F000Fu) | 0x43004300u, 0x3F803F80u, 0xC308C308u); }
 // code * scale rounded to bf16 as the stored value is defined.  The fp32 scale enters as two bf16 parts; the product
 // with the small part is rounded to 8 bits at 2^-8 of the value, so the sum's one rounding sees the product to 2^-17.
 __device__ __forceinline__ uint32_t q4_value(uint32_t code2, uint32_t hi2, uint32_t lo2) { return hfma2(code2, hi2, hmul2(code2, lo2)); }
@@ -108,15 +103,18 @@ __device__ __forceinline__ void split_scale(float s, uint32_t& hi2, uint32_t& lo
     lo2 = lu | (lu << 16);
 }
 
-template <int D, int Q, int ROWS>
+// How a tile of one item lies in shared memory.  Four computing warps share a tile, WT tokens each.
+template <int D, int Q>
 struct Layout {
     static constexpr int ROW = Q == IZB_KV_NONE ? 2 * D : Q == IZB_KV_INT8 ? D : D / 2;  // bytes of a token's K (or V)
     static constexpr int CHUNKS = ROW / 16;
-    static constexpr int TILE_BYTES = SP_TILE * ROW;
-    static constexpr int SCALE_BYTES = Q == IZB_KV_Q4_0 ? SP_TILE * (D / 32) * 4 : 0;
+    static constexpr int WT = ROW == 256 ? 16 : 32;  // 16 to 32 KB a tile: two CTAs on an SM keep 64 KB and more on the way
+    static constexpr int TILE = 4 * WT;
+    static constexpr int TILE_BYTES = TILE * ROW;
+    static constexpr int SCALE_BYTES = Q == IZB_KV_Q4_0 ? TILE * (D / 32) * 4 : 0;
     static constexpr int STAGE = 2 * (TILE_BYTES + SCALE_BYTES);
-    // two CTAs share an SM (113 KB each): the ring takes what the query rows leave
-    static constexpr int STAGES = Q == IZB_KV_NONE ? (ROWS <= 32 ? 3 : 2) : Q == IZB_KV_INT8 ? (ROWS <= 64 ? 5 : 4) : 6;
+    // what two CTAs (D = 64: three) of an SM can hold
+    static constexpr int STAGES = D == 128 ? (STAGE > 24 * 1024 ? 3 : 4) : STAGE > 24 * 1024 ? 2 : STAGE > 12 * 1024 ? 3 : 4;
     // place of 16-byte chunk c of token row r: the chunk index is mixed with the row so that the eight lanes of a
     // shared-memory phase (ldmatrix: eight rows of one chunk; codes: two rows of four chunks) meet different banks
     static __device__ __forceinline__ int place(int r, int c) {
@@ -126,36 +124,66 @@ struct Layout {
     }
 };
 
-// shared memory of an item: query rows, table of token places, Int8 scales, cross-warp scratch, then the tile ring
-// (which the final exchange between warps reuses)
-template <int D, int ROWS, int Q>
+// shared memory of an item: query rows, table of token places, Int8 scales, then the tile ring, which the final
+// exchange between the warps reuses (rows of D + 4 floats: consecutive rows start four banks apart)
+template <int D, int MT, int Q>
 constexpr int item_smem(int chunk) {
-    const int ring = Layout<D, Q, ROWS>::STAGE * Layout<D, Q, ROWS>::STAGES;
-    const int exchange = 4 * 32 * D * 4;  // at most 32 rows from each of four warps
-    return ROWS * D * 2 + chunk * 4 + (Q == IZB_KV_INT8 ? chunk * 4 : 0) + 4 * 32 * 8 + (ring > exchange ? ring : exchange);
+    const int ring = Layout<D, Q>::STAGE * Layout<D, Q>::STAGES;
+    const int exchange = 4 * 16 * MT * (D + 4) * 4;
+    return 16 * MT * D * 2 + chunk * 4 + (Q == IZB_KV_INT8 ? chunk * 4 : 0) + (ring > exchange ? ring : exchange);
 }
 
-// One item: rows [row0, row0 + n_rows) of the query rows that meet KV head kh of `src` row `src_row`, tokens
-// [t0, t1).  WM warps side by side over the rows (16 * MT rows each), 4 / WM over the tokens of a tile.
-template <int D, int WM, int MT, int Q>
+// Registers.  A launch of (256 threads, CTAS per SM) gets LAUNCH registers a thread; 128 copying threads keep COPY_REGS
+// of them and 128 computing threads take the rest: COMPUTE + COPY_REGS = 2 LAUNCH.
+constexpr int COPY_REGS = 24;
+template <int D, int MT>
+struct Regs {
+    static constexpr int CTAS = D == 64 && MT == 1 ? 3 : 2;
+    static constexpr int LAUNCH = CTAS == 3 ? 80 : 128;
+    static constexpr int COMPUTE = 2 * LAUNCH - COPY_REGS;
+};
+
+struct ItemShared {
+    unsigned long long full[4], empty[4];
+    float2 wml[4][32];    // per warp and row: maximum and sum
+    float factor[4][32];  // per warp and row: weight in the joined result
+    int abort_flag;
+};
+
+// One item: n_rows (at most 16 MT) query rows from row0 that meet KV head kh of `src` row `src_row`, tokens [t0, t1).
+// Warps 0..3 compute, each on its share of every tile with a maximum, sum and accumulator of its own; warps 4..7
+// copy tiles ahead of them through a ring of stages (cp.async onto an mbarrier), so that no warp waits for another one;
+// registers the copying warps do not need go to the computing ones (setmaxnreg; their shares add up to the launch's).
+//   Scores and outputs are mma.sync products of 16 rows: with at most 32 rows a 128-row tensor-memory tile would be idle
+// for three quarters of its rows, while here a tile's fragments are read (or made from codes) exactly once.
+template <int D, int MT, int Q, int MT_LAUNCH>
 __device__ __forceinline__ void attend(const Params& p, const Source& src, int src_row, int kh, int seq0, int row0, int n_rows, int t0,
-                                       int t1, int chunk_slot, int chunks_total, uint8_t* smem) {
-    constexpr int WN = 4 / WM, ROWS = 16 * MT * WM, TOK = SP_TILE / WN, NT = TOK / 8, KS = D / 16, DT = D / 8;
-    using L = Layout<D, Q, ROWS>;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp % WM, wn = warp / WM;
+                                       int t1, int chunk_slot, int chunks_total, uint8_t* smem, ItemShared& sh) {
+    using L = Layout<D, Q>;
+    constexpr int ROWS = 16 * MT, WT = L::WT, NT = WT / 8, KS = D / 16, DT = D / 8;
+    constexpr bool Q_IN_REGS = MT * D <= 128;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int gq = lane >> 2, tq = lane & 3;
-    const int n_tok = t1 - t0, n_tiles = (n_tok + SP_TILE - 1) / SP_TILE;
+    const int n_tok = t1 - t0, n_tiles = (n_tok + L::TILE - 1) / L::TILE;
 
     uint8_t* sq = smem;
     uint32_t* place = reinterpret_cast<uint32_t*>(sq + ROWS * D * 2);
-    uint32_t* tok_scale = place + src.chunk;                                     // Int8: bf16 (k, v) scales of each token
-    float2* wml = reinterpret_cast<float2*>(tok_scale + (Q == IZB_KV_INT8 ? src.chunk : 0));
-    uint8_t* ring = reinterpret_cast<uint8_t*>(wml + 4 * 32);
+    uint32_t* tok_scale = place + src.chunk;  // Int8: bf16 (k, v) scales of each token
+    uint8_t* ring = reinterpret_cast<uint8_t*>(tok_scale + (Q == IZB_KV_INT8 ? src.chunk : 0));
     const uint32_t ring_u = izb::smem_u32(ring), sq_u = izb::smem_u32(sq);
+    volatile int* abort_flag = &sh.abort_flag;
 
     // ---- where each token of the chunk lies, and the query rows ----
-    for (int i = tid; i < n_tiles * SP_TILE; i += SP_THREADS) {
-        uint32_t at = 0, sc = 0;
+    if (tid == 0) {
+        for (int s = 0; s < L::STAGES; ++s) {
+            izb::mbar_init(izb::smem_u32(&sh.full[s]), 128);
+            izb::mbar_init(izb::smem_u32(&sh.empty[s]), 4);
+        }
+        sh.abort_flag = 0;
+        izb::mbar_fence_init();
+    }
+    for (int i = tid; i < n_tiles * L::TILE; i += SP_THREADS) {
+        uint32_t at = 0, sc = 0;  // tokens past the chunk: a place that can be addressed, a zero scale
         if (i < n_tok) {
             const int t = t0 + i, pg = t / src.page_size;
             const int page = src.table[static_cast<long long>(src_row) * src.max_pages + pg];
@@ -171,320 +199,378 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
         if (r < n_rows) {
             const int s = row / p.g, h = row - s * p.g;
             v = *reinterpret_cast<const uint4*>(p.q + (seq0 + s) * p.ld_q + static_cast<long long>(kh * p.g + h) * D + c * 8);
+            v.x ^= p.q_sign; v.y ^= p.q_sign; v.z ^= p.q_sign; v.w ^= p.q_sign;
         }
+        // Q4_0 codes leave their words as the channel pairs (0, 4), (1, 5), (2, 6), (3, 7) of eight
+        if (Q == IZB_KV_Q4_0)
+            v = make_uint4(izb::prmt(v.x, v.z, 0x5410), izb::prmt(v.x, v.z, 0x7632), izb::prmt(v.y, v.w, 0x5410), izb::prmt(v.y, v.w, 0x7632));
         *reinterpret_cast<uint4*>(sq + r * D * 2 + ((c ^ (r & 7)) << 4)) = v;
     }
     __syncthreads();
 
-    auto issue = [&](int tile) {
-        if (tile < n_tiles) {
-            const uint32_t base = ring_u + (tile % L::STAGES) * L::STAGE;
-            const int tok0 = tile * SP_TILE;
-#pragma unroll
-            for (int j = 0; j < SP_TILE * L::CHUNKS / SP_THREADS; ++j) {
-                const int i = j * SP_THREADS + tid, r = i / L::CHUNKS, c = i % L::CHUNKS;
-                const bool ok = tok0 + r < n_tok;
-                const long long off =
-                    (static_cast<long long>(ok ? place[tok0 + r] : 0u) * p.kv_heads + kh) * L::ROW + c * 16;
-                cp16(base + L::place(r, c), src.k + (ok ? off : 0), ok);
-                cp16(base + L::TILE_BYTES + L::place(r, c), src.v + (ok ? off : 0), ok);
+    bool ok = true;
+    if (warp >= 4) {
+        // ---------------- copies ----------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(COPY_REGS));
+        const int t = tid - 128;
+        constexpr int RSTEP = 128 / L::CHUNKS;  // rows the 128 threads take at a time, a 16-byte chunk each
+        const int my_r = t / L::CHUNKS, my_c = t % L::CHUNKS;
+        const uint32_t stride = static_cast<uint32_t>(p.kv_heads) * L::ROW;
+        const uint8_t* k_from = src.k + kh * L::ROW + my_c * 16;
+        const uint8_t* v_from = src.v + kh * L::ROW + my_c * 16;
+        for (int tile = 0; tile < n_tiles; ++tile) {
+            const int stage = tile % L::STAGES;
+            if (!izb::mbar_wait_bounded(izb::smem_u32(&sh.empty[stage]), ((tile / L::STAGES) & 1) ^ 1, abort_flag)) {
+                ok = false;
+                break;
+            }
+            const uint32_t base = ring_u + stage * L::STAGE;
+            const int tok0 = tile * L::TILE;
+            // rows past the chunk become zeros as far as a product step of 16 tokens reaches
+            const int have = n_tok - tok0, need = min(L::TILE, (have + 15) & ~15);
+#pragma unroll 4
+            for (int j = 0; j < L::TILE / RSTEP; ++j) {
+                const int r = j * RSTEP + my_r;
+                if (r >= need) break;
+                const uint64_t off = static_cast<uint64_t>(place[tok0 + r]) * stride;
+                const int bytes = r < have ? 16 : 0;
+                const uint32_t dst = base + L::place(r, my_c);
+                cp16(dst, k_from + off, bytes);
+                cp16(dst + L::TILE_BYTES, v_from + off, bytes);
             }
             if (Q == IZB_KV_Q4_0) {
                 constexpr int B = D / 32;
-#pragma unroll
-                for (int j = 0; j < SP_TILE * B / SP_THREADS; ++j) {
-                    const int i = j * SP_THREADS + tid, r = i / B, c = i % B;
-                    const bool ok = tok0 + r < n_tok;
-                    const long long off = (static_cast<long long>(ok ? place[tok0 + r] : 0u) * p.kv_heads + kh) * B + c;
-                    cp4(base + 2 * L::TILE_BYTES + i * 4, src.k_scales + (ok ? off : 0), ok);
-                    cp4(base + 2 * L::TILE_BYTES + L::SCALE_BYTES + i * 4, src.v_scales + (ok ? off : 0), ok);
+#pragma unroll 4
+                for (int j = 0; j < L::TILE * B / 128; ++j) {
+                    const int i = j * 128 + t, r = i / B, c = i % B;
+                    const int bytes = r < have ? 4 : 0;
+                    const uint64_t off = static_cast<uint64_t>(place[tok0 + r]) * static_cast<uint32_t>(p.kv_heads * B) + static_cast<uint32_t>(kh * B + c);
+                    cp4(base + 2 * L::TILE_BYTES + i * 4, src.k_scales + off, bytes);
+                    cp4(base + 2 * L::TILE_BYTES + L::SCALE_BYTES + i * 4, src.v_scales + off, bytes);
                 }
             }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(izb::smem_u32(&sh.full[stage])) : "memory");
         }
-        cp_commit();
-    };
-#pragma unroll
-    for (int s = 0; s < L::STAGES - 1; ++s) issue(s);
-
-    float o[MT][DT][4], m[MT][2], l[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        m[mt][0] = m[mt][1] = -INFINITY;
-        l[mt][0] = l[mt][1] = 0.f;
-#pragma unroll
-        for (int j = 0; j < DT; ++j) o[mt][j][0] = o[mt][j][1] = o[mt][j][2] = o[mt][j][3] = 0.f;
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (!ok && lane == 0) atomicExch(p.status, 1);
+        return;
     }
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<D, MT_LAUNCH>::COMPUTE));
+    float o[MT][DT][4], m[MT][2], l[MT][2];
+    {
+        uint32_t qa[Q_IN_REGS ? MT : 1][Q_IN_REGS ? KS : 1][4];
+        // fragment of query rows 16 mt.. for product step ks.  bf16: channels in order (ldmatrix); codes: the order of d
+        // inside a product is free as long as both operands use it, lane tq takes the D / 4 channels from tq * D / 4, four
+        // of them per step, so that it finds a token's codes for all steps in consecutive bytes
+        auto q_frag = [&](uint32_t (&a)[4], int mt, int ks) {
+            if constexpr (Q == IZB_KV_NONE) {
+                const int r = mt * 16 + (lane & 15), c = ks * 2 + (lane >> 4);
+                ldsm4(a, sq_u + r * D * 2 + ((c ^ (r & 7)) << 4));
+            } else {
+                const int r = mt * 16 + gq, e = tq * (D / 4) + ks * 4, c = e >> 3;
+                const uint32_t at = sq_u + r * D * 2 + ((c ^ (r & 7)) << 4) + (e & 4) * 2;
+                const uint2 lo = izb::lds64(at), hi = izb::lds64(at + 8 * D * 2);
+                a[0] = lo.x; a[1] = hi.x; a[2] = lo.y; a[3] = hi.y;
+            }
+        };
+        if constexpr (Q_IN_REGS) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) q_frag(qa[mt][ks], mt, ks);
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            m[mt][0] = m[mt][1] = -INFINITY;
+            l[mt][0] = l[mt][1] = 0.f;
+#pragma unroll
+            for (int j = 0; j < DT; ++j) o[mt][j][0] = o[mt][j][1] = o[mt][j][2] = o[mt][j][3] = 0.f;
+        }
+        const int wt = warp * WT;  // this warp's first token in a tile
 
-    for (int tile = 0; tile < n_tiles; ++tile) {
-        cp_wait<L::STAGES - 2>();
-        __syncthreads();
-        issue(tile + L::STAGES - 1);
-        const uint32_t kt = ring_u + (tile % L::STAGES) * L::STAGE, vt = kt + L::TILE_BYTES;
-        const int wt = wn * TOK;  // this warp's first token in the tile
+        for (int tile = 0; tile < n_tiles; ++tile) {
+            const int stage = tile % L::STAGES;
+            if (!izb::mbar_wait_bounded(izb::smem_u32(&sh.full[stage]), (tile / L::STAGES) & 1, abort_flag)) {
+                ok = false;
+                break;
+            }
+            const uint32_t kt = ring_u + stage * L::STAGE, vt = kt + L::TILE_BYTES;
+            const int left = n_tok - tile * L::TILE - wt;  // tokens of this warp's share that exist
+            if (left > 0) {
+                // ---- scores: S[rows, tokens] = Q K^T ----
+                float s[MT][NT][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) s[mt][j][0] = s[mt][j][1] = s[mt][j][2] = s[mt][j][3] = 0.f;
+#pragma unroll
+                for (int j = 0; j < NT; j += 2) {
+                    if (j * 8 >= left) break;
+                    if constexpr (Q == IZB_KV_NONE) {
+                        const int r = wt + j * 8 + (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+                        for (int ks = 0; ks < KS; ++ks) {
+                            uint32_t b[4];
+                            ldsm4(b, kt + L::place(r, ks * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) {
+                                uint32_t t[4];
+                                if constexpr (!Q_IN_REGS) q_frag(t, mt, ks);
+                                const uint32_t(&a)[4] = Q_IN_REGS ? qa[Q_IN_REGS ? mt : 0][Q_IN_REGS ? ks : 0] : t;
+                                izb::mma_bf16_16816(s[mt][j], a[0], a[1], a[2], a[3], b[0], b[1]);
+                                izb::mma_bf16_16816(s[mt][j + 1], a[0], a[1], a[2], a[3], b[2], b[3]);
+                            }
+                        }
+                    } else {
+                        uint32_t b[2][KS * 2];
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+                            const int r = wt + (j + n) * 8 + gq;
+                            if constexpr (Q == IZB_KV_INT8) {
+                                const uint32_t sc = tok_scale[tile * L::TILE + r], sc2 = izb::prmt(sc, sc, 0x1010);
+#pragma unroll
+                                for (int h = 0; h < D / 64; ++h) {
+                                    const uint4 w = izb::lds128(kt + L::place(r, tq * (D / 64) + h));
+                                    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        b[n][h * 8 + i * 2] = hmul2(int8_pair(izb::prmt(x[i], 0u, 0x4140)), sc2);
+                                        b[n][h * 8 + i * 2 + 1] = hmul2(int8_pair(izb::prmt(x[i], 0u, 0x4342)), sc2);
+                                    }
+                                }
+                            } else {
+                                uint32_t hi2, lo2;
+                                split_scale(lds_f32(kt + 2 * L::TILE_BYTES + (r * (D / 32) + tq * (D / 4) / 32) * 4), hi2, lo2);
+                                uint32_t x[D / 32];
+                                if constexpr (D == 128) {
+                                    const uint4 w = izb::lds128(kt + L::place(r, tq));
+                                    x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w;
+                                } else {
+                                    const uint2 w = izb::lds64(kt + L::place(r, tq >> 1) + (tq & 1) * 8);
+                                    x[0] = w.x; x[1] = w.y;
+                                }
+#pragma unroll
+                                for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) b[n][i * 4 + e] = q4_value(q4_pair(x[i] >> (4 * e)), hi2, lo2);
+                            }
+                        }
+#pragma unroll
+                        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) {
+                                uint32_t t[4];
+                                if constexpr (!Q_IN_REGS) q_frag(t, mt, ks);
+                                const uint32_t(&a)[4] = Q_IN_REGS ? qa[Q_IN_REGS ? mt : 0][Q_IN_REGS ? ks : 0] : t;
+                                izb::mma_bf16_16816(s[mt][j], a[0], a[1], a[2], a[3], b[0][ks * 2], b[0][ks * 2 + 1]);
+                                izb::mma_bf16_16816(s[mt][j + 1], a[0], a[1], a[2], a[3], b[1][ks * 2], b[1][ks * 2 + 1]);
+                            }
+                    }
+                }
 
-        // ---- scores: S[rows, tokens] = Q K^T ----
-        float s[MT][NT][4];
+                // ---- running maximum and sum; s becomes the weights ----
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    if (left < WT) {
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (j * 8 + tq * 2 + (e & 1) >= left) s[mt][j][e] = -INFINITY;
+                    }
+                    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[mt][j][e]);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xFFFFFFFFu, mx[h], 1));
+                        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xFFFFFFFFu, mx[h], 2));
+                    }
+                    // The reference point of a row follows its maximum only when that has grown by 2^8: weights up to 2^8
+                    // are as exact as weights up to 1, and the accumulators are seldom rescaled.  (Not-less: also for the
+                    // first maximum.)
+                    if (__any_sync(0xFFFFFFFFu, !(mx[0] <= m[mt][0] + p.margin) || !(mx[1] <= m[mt][1] + p.margin))) {
+                        float f[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float n = fmaxf(m[mt][h], mx[h]);
+                            f[h] = m[mt][h] == -INFINITY ? 0.f : ex2((m[mt][h] - n) * p.scale_log2);
+                            m[mt][h] = n;
+                            l[mt][h] *= f[h];
+                        }
+#pragma unroll
+                        for (int j = 0; j < DT; ++j) {
+                            o[mt][j][0] *= f[0]; o[mt][j][1] *= f[0];
+                            o[mt][j][2] *= f[1]; o[mt][j][3] *= f[1];
+                        }
+                    }
+                    // no token yet: nothing is subtracted, so that exp2(-inf) gives the zero weight
+                    const float u0 = m[mt][0] == -INFINITY ? 0.f : m[mt][0] * p.scale_log2, u1 = m[mt][1] == -INFINITY ? 0.f : m[mt][1] * p.scale_log2;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        s[mt][j][0] = ex2(fmaf(s[mt][j][0], p.scale_log2, -u0));
+                        s[mt][j][1] = ex2(fmaf(s[mt][j][1], p.scale_log2, -u0));
+                        s[mt][j][2] = ex2(fmaf(s[mt][j][2], p.scale_log2, -u1));
+                        s[mt][j][3] = ex2(fmaf(s[mt][j][3], p.scale_log2, -u1));
+                        l[mt][0] += s[mt][j][0] + s[mt][j][1];
+                        l[mt][1] += s[mt][j][2] + s[mt][j][3];
+                    }
+                }
+
+                // ---- O += P V, sixteen tokens a step ----
+#pragma unroll
+                for (int k16 = 0; k16 < NT / 2; ++k16) {
+                    if (k16 * 16 >= left) break;
+                    uint32_t a[MT][4];
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        a[mt][0] = izb::pack_bf16x2(s[mt][2 * k16][0], s[mt][2 * k16][1]);
+                        a[mt][1] = izb::pack_bf16x2(s[mt][2 * k16][2], s[mt][2 * k16][3]);
+                        a[mt][2] = izb::pack_bf16x2(s[mt][2 * k16 + 1][0], s[mt][2 * k16 + 1][1]);
+                        a[mt][3] = izb::pack_bf16x2(s[mt][2 * k16 + 1][2], s[mt][2 * k16 + 1][3]);
+                    }
+                    auto accumulate = [&](int j, uint32_t b0, uint32_t b1) {
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) izb::mma_bf16_16816(o[mt][j], a[mt][0], a[mt][1], a[mt][2], a[mt][3], b0, b1);
+                    };
+                    if constexpr (Q == IZB_KV_NONE) {
+#pragma unroll
+                        for (int j = 0; j < DT; j += 2) {
+                            uint32_t b[4];
+                            ldsm4t(b, vt + L::place(wt + k16 * 16 + (lane & 15), j + (lane >> 4)));
+                            accumulate(j, b[0], b[1]);
+                            accumulate(j + 1, b[2], b[3]);
+                        }
+                    } else {
+                        // column n of output tile j stands for channel n * (D / 8) + j, so that a lane (n = gq) takes D / 8
+                        // consecutive channels of its four tokens and pairs tokens 2 tq and 2 tq + 1 (and + 8) code by code
+                        const int r0 = wt + k16 * 16 + tq * 2;
+                        const int rows[4] = {r0, r0 + 1, r0 + 8, r0 + 9};
+                        uint32_t x[4][4];  // the D / 8 codes of each token
+                        if constexpr (Q == IZB_KV_INT8) {
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) {
+                                if constexpr (D == 128) {
+                                    const uint4 w = izb::lds128(vt + L::place(rows[t], gq));
+                                    x[t][0] = w.x; x[t][1] = w.y; x[t][2] = w.z; x[t][3] = w.w;
+                                } else {
+                                    const uint2 w = izb::lds64(vt + L::place(rows[t], gq >> 1) + (gq & 1) * 8);
+                                    x[t][0] = w.x; x[t][1] = w.y;
+                                }
+                            }
+                            const uint32_t* ts = tok_scale + tile * L::TILE;
+                            const uint32_t s01 = izb::prmt(ts[rows[0]], ts[rows[1]], 0x7632), s23 = izb::prmt(ts[rows[2]], ts[rows[3]], 0x7632);
+#pragma unroll
+                            for (int j = 0; j < DT; ++j) {
+                                const int w = j >> 2, by = j & 3;
+                                const uint32_t sel = by | ((4 + by) << 8);  // byte `by` of both words; int8_pair masks the rest
+                                accumulate(j, hmul2(int8_pair(izb::prmt(x[0][w], x[1][w], sel)), s01),
+                                           hmul2(int8_pair(izb::prmt(x[2][w], x[3][w], sel)), s23));
+                            }
+                        } else {
+                            const int blk = gq * (D / 8) / 32;
+                            float sc[4];
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) {
+                                sc[t] = lds_f32(kt + 2 * L::TILE_BYTES + L::SCALE_BYTES + (rows[t] * (D / 32) + blk) * 4);
+                                if constexpr (D == 128) {
+                                    const uint2 w = izb::lds64(vt + L::place(rows[t], gq >> 1) + (gq & 1) * 8);
+                                    x[t][0] = w.x; x[t][1] = w.y;
+                                } else {
+                                    x[t][0] = izb::lds32(vt + L::place(rows[t], gq >> 2) + (gq & 3) * 4);
+                                }
+                            }
+                            uint32_t ha, la, hb, lb;
+                            split_scale(sc[0], ha, la);
+                            split_scale(sc[1], hb, lb);
+                            const uint32_t h01 = izb::prmt(ha, hb, 0x5410), l01 = izb::prmt(la, lb, 0x5410);
+                            split_scale(sc[2], ha, la);
+                            split_scale(sc[3], hb, lb);
+                            const uint32_t h23 = izb::prmt(ha, hb, 0x5410), l23 = izb::prmt(la, lb, 0x5410);
+#pragma unroll
+                            for (int j = 0; j < DT; ++j) {
+                                const uint32_t sel = (j & 4) ? 0x7632u : 0x5410u;  // four codes of both tokens side by side
+                                const uint32_t w01 = izb::prmt(x[0][j >> 3], x[1][j >> 3], sel), w23 = izb::prmt(x[2][j >> 3], x[3][j >> 3], sel);
+                                accumulate(j, q4_value(q4_pair(w01 >> (4 * (j & 3))), h01, l01), q4_value(q4_pair(w23 >> (4 * (j & 3))), h23, l23));
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) izb::mbar_arrive(izb::smem_u32(&sh.empty[stage]));
+        }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) s[mt][j][0] = s[mt][j][1] = s[mt][j][2] = s[mt][j][3] = 0.f;
-        if constexpr (Q == IZB_KV_NONE) {
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                uint32_t a[MT][4];
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    const int r = (wm * MT + mt) * 16 + (lane & 15), c = ks * 2 + (lane >> 4);
-                    ldsm4(a[mt], sq_u + r * D * 2 + ((c ^ (r & 7)) << 4));
-                }
-#pragma unroll
-                for (int j = 0; j < NT; j += 2) {
-                    uint32_t b[4];
-                    const int r = wt + j * 8 + (lane & 7) + ((lane >> 4) << 3), c = ks * 2 + ((lane >> 3) & 1);
-                    ldsm4(b, kt + L::place(r, c));
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        izb::mma_bf16_16816(s[mt][j], a[mt][0], a[mt][1], a[mt][2], a[mt][3], b[0], b[1]);
-                        izb::mma_bf16_16816(s[mt][j + 1], a[mt][0], a[mt][1], a[mt][2], a[mt][3], b[2], b[3]);
-                    }
-                }
+            for (int h = 0; h < 2; ++h) {
+                l[mt][h] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][h], 1);
+                l[mt][h] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][h], 2);
+                if (tq == 0) sh.wml[warp][mt * 16 + h * 8 + gq] = make_float2(m[mt][h], l[mt][h]);
             }
-        } else {
-            // Codes become fragments in registers.  The order of d inside a product is free as long as both operands
-            // use it: lane tq takes the D / 4 consecutive channels from tq * D / 4, four of them per mma step.
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const int r = wt + j * 8 + gq;
-                uint32_t b[KS * 2];
-                if constexpr (Q == IZB_KV_INT8) {
-                    const uint32_t sc = tok_scale[tile * SP_TILE + r];
-                    const uint32_t sc2 = izb::prmt(sc, sc, 0x1010);
-#pragma unroll
-                    for (int h = 0; h < D / 64; ++h) {
-                        const uint4 w = izb::lds128(kt + L::place(r, tq * (D / 64) + h));
-                        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            b[h * 8 + i * 2] = hmul2(int8_pair(izb::prmt(x[i], 0u, 0x4140)), sc2);
-                            b[h * 8 + i * 2 + 1] = hmul2(int8_pair(izb::prmt(x[i], 0u, 0x4342)), sc2);
-                        }
-                    }
-                } else {
-                    const int blk = tq * (D / 4) / 32;
-                    uint32_t hi2, lo2;
-                    split_scale(lds_f32(kt + 2 * L::TILE_BYTES + (r * (D / 32) + blk) * 4), hi2, lo2);
-                    uint32_t x[D / 32];
-                    if constexpr (D == 128) {
-                        const uint4 w = izb::lds128(kt + L::place(r, tq));
-                        x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w;
-                    } else {
-                        const uint2 w = izb::lds64(kt + L::place(r, tq >> 1) + (tq & 1) * 8);
-                        x[0] = w.x; x[1] = w.y;
-                    }
-                    // eight codes of a word, low nibble first: byte i holds channels 2 i and 2 i + 1
-#pragma unroll
-                    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t by = (x[i] >> (8 * e)) & 0xFFu;
-                            b[i * 4 + e] = q4_value(q4_pair(by | (by << 12)), hi2, lo2);
-                        }
-                }
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    const int r0 = (wm * MT + mt) * 16 + gq;
-#pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        const int e = tq * (D / 4) + ks * 4, c = e >> 3, half = (e & 4) * 2;
-                        const uint2 a0 = izb::lds64(sq_u + r0 * D * 2 + ((c ^ (r0 & 7)) << 4) + half);
-                        const uint2 a1 = izb::lds64(sq_u + (r0 + 8) * D * 2 + ((c ^ (r0 & 7)) << 4) + half);
-                        izb::mma_bf16_16816(s[mt][j], a0.x, a1.x, a0.y, a1.y, b[ks * 2], b[ks * 2 + 1]);
-                    }
-                }
-            }
-        }
-
-        // ---- running maximum and sum; s becomes the weights ----
-        const int left = n_tok - tile * SP_TILE - wt;  // tokens of this warp's share that exist
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const bool in = j * 8 + tq * 2 + (e & 1) < left;
-                    s[mt][j][e] = in ? s[mt][j][e] * p.scale_log2 : -INFINITY;
-                    if (e < 2) mx0 = fmaxf(mx0, s[mt][j][e]);
-                    else mx1 = fmaxf(mx1, s[mt][j][e]);
-                }
-            mx0 = fmaxf(mx0, __shfl_xor_sync(0xFFFFFFFFu, mx0, 1));
-            mx0 = fmaxf(mx0, __shfl_xor_sync(0xFFFFFFFFu, mx0, 2));
-            mx1 = fmaxf(mx1, __shfl_xor_sync(0xFFFFFFFFu, mx1, 1));
-            mx1 = fmaxf(mx1, __shfl_xor_sync(0xFFFFFFFFu, mx1, 2));
-            const float n0 = fmaxf(m[mt][0], mx0), n1 = fmaxf(m[mt][1], mx1);
-            // no token yet: subtract 0 so that exp2(-inf) gives the zero weight
-            const float u0 = n0 == -INFINITY ? 0.f : n0, u1 = n1 == -INFINITY ? 0.f : n1;
-            if (__any_sync(0xFFFFFFFFu, n0 != m[mt][0] || n1 != m[mt][1])) {
-                const float f0 = ex2(m[mt][0] - u0), f1 = ex2(m[mt][1] - u1);
-                l[mt][0] *= f0;
-                l[mt][1] *= f1;
-#pragma unroll
-                for (int j = 0; j < DT; ++j) {
-                    o[mt][j][0] *= f0; o[mt][j][1] *= f0;
-                    o[mt][j][2] *= f1; o[mt][j][3] *= f1;
-                }
-                m[mt][0] = n0;
-                m[mt][1] = n1;
-            }
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                s[mt][j][0] = ex2(s[mt][j][0] - u0);
-                s[mt][j][1] = ex2(s[mt][j][1] - u0);
-                s[mt][j][2] = ex2(s[mt][j][2] - u1);
-                s[mt][j][3] = ex2(s[mt][j][3] - u1);
-                l[mt][0] += s[mt][j][0] + s[mt][j][1];
-                l[mt][1] += s[mt][j][2] + s[mt][j][3];
-            }
-        }
-
-        // ---- O += P V, sixteen tokens a step ----
-#pragma unroll
-        for (int kt16 = 0; kt16 < NT / 2; ++kt16) {
-            uint32_t a[MT][4];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                a[mt][0] = izb::pack_bf16x2(s[mt][2 * kt16][0], s[mt][2 * kt16][1]);
-                a[mt][1] = izb::pack_bf16x2(s[mt][2 * kt16][2], s[mt][2 * kt16][3]);
-                a[mt][2] = izb::pack_bf16x2(s[mt][2 * kt16 + 1][0], s[mt][2 * kt16 + 1][1]);
-                a[mt][3] = izb::pack_bf16x2(s[mt][2 * kt16 + 1][2], s[mt][2 * kt16 + 1][3]);
-            }
-            if constexpr (Q == IZB_KV_NONE) {
-#pragma unroll
-                for (int j = 0; j < DT; j += 2) {
-                    uint32_t b[4];
-                    const int r = wt + kt16 * 16 + (lane & 15), c = j + (lane >> 4);
-                    ldsm4t(b, vt + L::place(r, c));
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        izb::mma_bf16_16816(o[mt][j], a[mt][0], a[mt][1], a[mt][2], a[mt][3], b[0], b[1]);
-                        izb::mma_bf16_16816(o[mt][j + 1], a[mt][0], a[mt][1], a[mt][2], a[mt][3], b[2], b[3]);
-                    }
-                }
-            } else {
-                // column n of output tile j stands for channel n * (D / 8) + j, so that a lane (n = gq) takes D / 8
-                // consecutive channels of its four tokens and pairs tokens 2 tq and 2 tq + 1 (and + 8) byte by byte
-                const int r0 = wt + kt16 * 16 + tq * 2;
-                const int rows[4] = {r0, r0 + 1, r0 + 8, r0 + 9};
-                uint32_t x[4][4];  // the D / 8 codes of each token
-                uint32_t h01, l01, h23, l23;
-                if constexpr (Q == IZB_KV_INT8) {
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        if constexpr (D == 128) {
-                            const uint4 w = izb::lds128(vt + L::place(rows[t], gq));
-                            x[t][0] = w.x; x[t][1] = w.y; x[t][2] = w.z; x[t][3] = w.w;
-                        } else {
-                            const uint2 w = izb::lds64(vt + L::place(rows[t], gq >> 1) + (gq & 1) * 8);
-                            x[t][0] = w.x; x[t][1] = w.y;
-                        }
-                    }
-                    const uint32_t* ts = tok_scale + tile * SP_TILE;
-                    h01 = izb::prmt(ts[rows[0]], ts[rows[1]], 0x7632);
-                    h23 = izb::prmt(ts[rows[2]], ts[rows[3]], 0x7632);
-                    l01 = l23 = 0u;
-#pragma unroll
-                    for (int j = 0; j < DT; ++j) {
-                        const int w = j >> 2, by = j & 3;
-                        const uint32_t sel = by | ((4 + by) << 8);  // byte `by` of both words; int8_pair masks the rest
-                        const uint32_t b0 = hmul2(int8_pair(izb::prmt(x[0][w], x[1][w], sel)), h01);
-                        const uint32_t b1 = hmul2(int8_pair(izb::prmt(x[2][w], x[3][w], sel)), h23);
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt)
-                            izb::mma_bf16_16816(o[mt][j], a[mt][0], a[mt][1], a[mt][2], a[mt][3], b0, b1);
-                    }
-                } else {
-                    const int blk = gq * (D / 8) / 32;
-                    float sc[4];
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        sc[t] = lds_f32(kt + 2 * L::TILE_BYTES + L::SCALE_BYTES + (rows[t] * (D / 32) + blk) * 4);
-                        if constexpr (D == 128) {
-                            const uint2 w = izb::lds64(vt + L::place(rows[t], gq >> 1) + (gq & 1) * 8);
-                            x[t][0] = w.x; x[t][1] = w.y;
-                        } else {
-                            x[t][0] = izb::lds32(vt + L::place(rows[t], gq >> 2) + (gq & 3) * 4);
-                        }
-                    }
-                    uint32_t ha, la, hb, lb;
-                    split_scale(sc[0], ha, la); split_scale(sc[1], hb, lb);
-                    h01 = izb::prmt(ha, hb, 0x5410); l01 = izb::prmt(la, lb, 0x5410);
-                    split_scale(sc[2], ha, la); split_scale(sc[3], hb, lb);
-                    h23 = izb::prmt(ha, hb, 0x5410); l23 = izb::prmt(la, lb, 0x5410);
-#pragma unroll
-                    for (int j = 0; j < DT; ++j) {
-                        const int w = j >> 3, sh = 4 * (j & 7);
-                        const uint32_t b0 = q4_value(q4_pair(((x[0][w] >> sh) & 0xFu) | (((x[1][w] >> sh) & 0xFu) << 16)), h01, l01);
-                        const uint32_t b1 = q4_value(q4_pair(((x[2][w] >> sh) & 0xFu) | (((x[3][w] >> sh) & 0xFu) << 16)), h23, l23);
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt)
-                            izb::mma_bf16_16816(o[mt][j], a[mt][0], a[mt][1], a[mt][2], a[mt][3], b0, b1);
-                    }
-                }
-            }
-        }
     }
-    cp_wait<0>();
+    if (!ok && lane == 0) atomicExch(p.status, 1);
+    izb::named_bar_sync(1, 128);  // every tile of the ring has been read; from here on the four computing warps alone
 
-    // ---- join the warps that shared the rows, leave the chunk's result ----
+    // ---- join the warps, leave the chunk's result ----
+    constexpr int LD = D + 4;
+    float* ex = reinterpret_cast<float*>(ring);  // [warp][16 MT][LD]
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            l[mt][h] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][h], 1);
-            l[mt][h] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][h], 2);
-            if (tq == 0) wml[warp * 32 + mt * 16 + h * 8 + gq] = make_float2(m[mt][h], l[mt][h]);
-        }
-    __syncthreads();  // also: every tile of the ring has been read
-    float* ex = reinterpret_cast<float*>(ring);  // [warp][16 MT][D]
+            float* row = ex + (warp * ROWS + mt * 16 + h * 8 + gq) * LD;
+            if constexpr (Q == IZB_KV_NONE) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+                for (int j = 0; j < DT; ++j) *reinterpret_cast<float2*>(row + j * 8 + tq * 2) = make_float2(o[mt][j][h * 2], o[mt][j][h * 2 + 1]);
+            } else {
 #pragma unroll
-        for (int j = 0; j < DT; ++j)
+                for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = mt * 16 + gq + (e >> 1) * 8;
-                const int n = tq * 2 + (e & 1);
-                const int d = Q == IZB_KV_NONE ? j * 8 + n : n * DT + j;
-                ex[(warp * 16 * MT + r) * D + d] = o[mt][j][e];
+                    for (int j = 0; j < DT; j += 4)
+                        *reinterpret_cast<float4*>(row + (tq * 2 + e) * DT + j) =
+                            make_float4(o[mt][j][h * 2 + e], o[mt][j + 1][h * 2 + e], o[mt][j + 2][h * 2 + e], o[mt][j + 3][h * 2 + e]);
             }
-    __syncthreads();
-    for (int i = tid; i < n_rows * D; i += SP_THREADS) {
-        const int r = i / D, d = i - r * D;
-        const int w = r / (16 * MT), rr = r - w * 16 * MT;
-        float top = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < WN; ++n) top = fmaxf(top, wml[(n * WM + w) * 32 + rr].x);
-        float sum = 0.f, a = 0.f;
-#pragma unroll
-        for (int n = 0; n < WN; ++n) {
-            const float2 x = wml[(n * WM + w) * 32 + rr];
-            const float f = x.x == -INFINITY ? 0.f : ex2(x.x - top);
-            sum += f * x.y;
-            a += f * ex[((n * WM + w) * 16 * MT + rr) * D + d];
         }
-        const int row = row0 + r, sq_i = row / p.g, h = row - sq_i * p.g;
-        const long long slot = (static_cast<long long>(seq0 + sq_i) * p.heads + kh * p.g + h) * chunks_total + chunk_slot;
-        p.acc[slot * D + d] = a;
-        if (d == 0) p.ml[slot] = make_float2(top, sum);
+    auto slot_of = [&](int r) {
+        const int row = row0 + r, s = row / p.g, h = row - s * p.g;
+        return (static_cast<long long>(seq0 + s) * p.heads + kh * p.g + h) * chunks_total + chunk_slot;
+    };
+    if (tid < n_rows) {
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, sh.wml[w][tid].x);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float2 x = sh.wml[w][tid];
+            const float f = x.x == -INFINITY ? 0.f : ex2((x.x - top) * p.scale_log2);
+            sh.factor[w][tid] = f;
+            sum += f * x.y;
+        }
+        p.ml[slot_of(tid)] = make_float2(top * p.scale_log2, sum);
+    }
+    izb::named_bar_sync(1, 128);
+    for (int i = tid; i < n_rows * (D / 4); i += 128) {
+        const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = sh.factor[w][r];
+            const float4 x = *reinterpret_cast<const float4*>(ex + (w * ROWS + r) * LD + d);
+            a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
+        }
+        *reinterpret_cast<float4*>(p.acc + slot_of(r) * D + d) = a;
     }
 }
 
 __device__ __forceinline__ int length_of(const Source& s, int row) { return min(max(s.lens[row], 0), s.max_len); }
 
-template <int D, int WM, int MT>
-__global__ void __launch_bounds__(SP_THREADS) shared_prefix_kernel(const __grid_constant__ Params p) {
+template <int D, int MT>
+__global__ void __launch_bounds__(SP_THREADS, Regs<D, MT>::CTAS) shared_prefix_kernel(const __grid_constant__ Params p) {
     extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ ItemShared sh;
     izb::pdl_launch_dependents();
     izb::pdl_wait();
     const int chunks = p.prefix.n_chunks + p.own.n_chunks;
@@ -498,14 +584,13 @@ __global__ void __launch_bounds__(SP_THREADS) shared_prefix_kernel(const __grid_
         const int chunk = item % p.prefix.n_chunks, group = item / p.prefix.n_chunks;
         const int len = length_of(p.prefix, group), t0 = chunk * p.prefix.chunk, t1 = min(len, t0 + p.prefix.chunk);
         if (t0 >= t1) return;
-        constexpr int ROWS = 16 * MT * WM;
-        const int row0 = rb * ROWS, n = min(ROWS, p.seqs * p.g - row0);
+        const int row0 = rb * 16 * MT, n = min(16 * MT, p.seqs * p.g - row0);
         if (p.prefix.quant == IZB_KV_NONE)
-            attend<D, WM, MT, IZB_KV_NONE>(p, p.prefix, group, kh, group * p.seqs, row0, n, t0, t1, chunk, chunks, smem);
+            attend<D, MT, IZB_KV_NONE, MT>(p, p.prefix, group, kh, group * p.seqs, row0, n, t0, t1, chunk, chunks, smem, sh);
         else if (p.prefix.quant == IZB_KV_INT8)
-            attend<D, WM, MT, IZB_KV_INT8>(p, p.prefix, group, kh, group * p.seqs, row0, n, t0, t1, chunk, chunks, smem);
+            attend<D, MT, IZB_KV_INT8, MT>(p, p.prefix, group, kh, group * p.seqs, row0, n, t0, t1, chunk, chunks, smem, sh);
         else
-            attend<D, WM, MT, IZB_KV_Q4_0>(p, p.prefix, group, kh, group * p.seqs, row0, n, t0, t1, chunk, chunks, smem);
+            attend<D, MT, IZB_KV_Q4_0, MT>(p, p.prefix, group, kh, group * p.seqs, row0, n, t0, t1, chunk, chunks, smem, sh);
         return;
     }
     item -= p.prefix_items;
@@ -515,9 +600,9 @@ __global__ void __launch_bounds__(SP_THREADS) shared_prefix_kernel(const __grid_
     const int len = length_of(p.own, seq), t0 = chunk * p.own.chunk, t1 = min(len, t0 + p.own.chunk);
     if (t0 >= t1) return;
     const int slot = p.prefix.n_chunks + chunk;
-    if (p.own.quant == IZB_KV_NONE) attend<D, 1, 1, IZB_KV_NONE>(p, p.own, seq, kh, seq, 0, p.g, t0, t1, slot, chunks, smem);
-    else if (p.own.quant == IZB_KV_INT8) attend<D, 1, 1, IZB_KV_INT8>(p, p.own, seq, kh, seq, 0, p.g, t0, t1, slot, chunks, smem);
-    else attend<D, 1, 1, IZB_KV_Q4_0>(p, p.own, seq, kh, seq, 0, p.g, t0, t1, slot, chunks, smem);
+    if (p.own.quant == IZB_KV_NONE) attend<D, 1, IZB_KV_NONE, MT>(p, p.own, seq, kh, seq, 0, p.g, t0, t1, slot, chunks, smem, sh);
+    else if (p.own.quant == IZB_KV_INT8) attend<D, 1, IZB_KV_INT8, MT>(p, p.own, seq, kh, seq, 0, p.g, t0, t1, slot, chunks, smem, sh);
+    else attend<D, 1, IZB_KV_Q4_0, MT>(p, p.own, seq, kh, seq, 0, p.g, t0, t1, slot, chunks, smem, sh);
 }
 
 // One CTA per (sequence, head): four warps take every fourth chunk, a lane D / 32 channels.
@@ -575,7 +660,7 @@ __global__ void __launch_bounds__(128)
 
 // ---- host side ---------------------------------------------------------------------------------------------------
 struct Plan {
-    int rows;        // query rows of a prefix item: 16, 32, 64 or 128
+    int rows;        // query rows of a prefix item: 16 or 32
     int row_blocks;
     int prefix_chunk, prefix_chunks, own_chunk, own_chunks;
 };
@@ -599,11 +684,12 @@ int choose_chunk(int64_t base, int64_t tokens, int64_t slots) {
     return static_cast<int>(best * SP_TILE);
 }
 
-Plan make_plan(const izb_ctx* ctx, int64_t groups, int64_t seqs, int kv_heads, int g, int64_t max_prefix, int64_t max_own) {
+Plan make_plan(const izb_ctx* ctx, int64_t groups, int64_t seqs, int kv_heads, int g, int head_dim, int64_t max_prefix, int64_t max_own) {
     Plan pl = {};
-    const int64_t rows = seqs * g, slots = 2 * static_cast<int64_t>(ctx && ctx->sm_count > 0 ? ctx->sm_count : 148);
+    const int64_t rows = seqs * g;
+    const int64_t slots = (head_dim == 64 && rows <= 16 ? 3 : 2) * static_cast<int64_t>(ctx && ctx->sm_count > 0 ? ctx->sm_count : 148);
     // the smallest block that holds the rows: a tile's fragments serve all rows of a block, idle rows cost mma steps
-    pl.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    pl.rows = rows <= 16 ? 16 : 32;
     pl.row_blocks = static_cast<int>((rows + pl.rows - 1) / pl.rows);
     if (max_prefix > 0) {
         pl.prefix_chunk = choose_chunk(groups * kv_heads * pl.row_blocks, max_prefix, slots);
@@ -645,23 +731,26 @@ int source_from(const izb_kv_pages* a, const int32_t* lens, int64_t max_len, Sou
     return IZB_OK;
 }
 
-template <int D, int ROWS>
+template <int D, int MT>
 size_t smem_for(const Source& s) {
     if (s.n_chunks == 0) return 0;
-    return s.quant == IZB_KV_NONE ? item_smem<D, ROWS, IZB_KV_NONE>(s.chunk)
-           : s.quant == IZB_KV_INT8 ? item_smem<D, ROWS, IZB_KV_INT8>(s.chunk) : item_smem<D, ROWS, IZB_KV_Q4_0>(s.chunk);
+    return s.quant == IZB_KV_NONE ? item_smem<D, MT, IZB_KV_NONE>(s.chunk)
+           : s.quant == IZB_KV_INT8 ? item_smem<D, MT, IZB_KV_INT8>(s.chunk) : item_smem<D, MT, IZB_KV_Q4_0>(s.chunk);
 }
 
-template <int D, int WM, int MT>
+template <int D, int MT>
 int launch_items(izb_ctx* ctx, cudaStream_t s, const Params& p, int64_t items) {
-    size_t smem = smem_for<D, 16 * MT * WM>(p.prefix);
-    const size_t own = smem_for<D, 16>(p.own);
+    size_t smem = smem_for<D, MT>(p.prefix);
+    const size_t own = smem_for<D, 1>(p.own);
     if (own > smem) smem = own;
-    auto kern = shared_prefix_kernel<D, WM, MT>;
-    static std::atomic<int> smem_set[IZB_MAX_DEVICES];
-    if (smem_set[ctx->device].load(std::memory_order_relaxed) < static_cast<int>(smem)) {
-        IZB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ctx->max_smem_optin));
-        smem_set[ctx->device].store(ctx->max_smem_optin, std::memory_order_relaxed);
+    auto kern = shared_prefix_kernel<D, MT>;
+    static std::atomic<bool> ready[IZB_MAX_DEVICES];
+    if (!ready[ctx->device].load(std::memory_order_relaxed)) {
+        cudaFuncAttributes attr;
+        IZB_CUDA_TRY(cudaFuncGetAttributes(&attr, kern));
+        if (attr.numRegs < Regs<D, MT>::LAUNCH) return IZB_ERR_LAUNCH;  // the computing warps would wait for registers nobody has
+        IZB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ctx->max_smem_optin - static_cast<int>(attr.sharedSizeBytes)));
+        ready[ctx->device].store(true, std::memory_order_relaxed);
     }
     IZB_CUDA_TRY(izb::launch_chained(ctx, kern, dim3(static_cast<unsigned>(items)), dim3(SP_THREADS), smem, s, p));
     ctx->launches.fetch_add(1, std::memory_order_relaxed);
@@ -672,10 +761,7 @@ template <int D>
 int launch_dim(izb_ctx* ctx, cudaStream_t s, const Params& p, const Plan& pl, int64_t items, int64_t batch, __nv_bfloat16* out,
                long long ld_out) {
     if (items > 0) {
-        const int rc = pl.rows == 16   ? launch_items<D, 1, 1>(ctx, s, p, items)
-                       : pl.rows == 32 ? launch_items<D, 1, 2>(ctx, s, p, items)
-                       : pl.rows == 64 ? launch_items<D, 2, 2>(ctx, s, p, items)
-                                       : launch_items<D, 4, 2>(ctx, s, p, items);
+        const int rc = pl.rows == 16 ? launch_items<D, 1>(ctx, s, p, items) : launch_items<D, 2>(ctx, s, p, items);
         if (rc != IZB_OK) return rc;
     }
     IZB_CUDA_TRY(izb::launch_chained(ctx, shared_prefix_join_kernel<D>, dim3(static_cast<unsigned>(batch * p.heads)), dim3(128), 0, s, p, out,
@@ -694,7 +780,7 @@ size_t izb_shared_prefix_decode_gqa_attention_workspace_bytes(const izb_ctx* ctx
     if (groups <= 0 || seqs_per_group <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || head_dim <= 0 ||
         max_prefix_len < 0 || max_seq_len < 0 || groups > INT32_MAX / seqs_per_group || max_prefix_len > INT32_MAX || max_seq_len > INT32_MAX)
         return 0;
-    const Plan pl = make_plan(ctx, groups, seqs_per_group, kv_heads, heads / kv_heads, max_prefix_len, max_seq_len);
+    const Plan pl = make_plan(ctx, groups, seqs_per_group, kv_heads, heads / kv_heads, head_dim, max_prefix_len, max_seq_len);
     return plan_bytes(pl, groups * seqs_per_group, heads, head_dim);
 }
 
@@ -721,7 +807,7 @@ int32_t izb_shared_prefix_decode_gqa_attention(izb_ctx* ctx, izb_stream stream, 
     if (ld_q < static_cast<int64_t>(heads) * d || ld_out < static_cast<int64_t>(heads) * d) return IZB_ERR_BAD_ARG;
     if (groups > INT32_MAX / seqs_per_group || groups * seqs_per_group > INT32_MAX / heads) return IZB_ERR_UNSUPPORTED;
     const int64_t batch = groups * seqs_per_group;
-    const Plan pl = make_plan(ctx, groups, seqs_per_group, kv_heads, heads / kv_heads, max_prefix_len, max_seq_len);
+    const Plan pl = make_plan(ctx, groups, seqs_per_group, kv_heads, heads / kv_heads, d, max_prefix_len, max_seq_len);
     const size_t need = plan_bytes(pl, batch, heads, d);
     if (need && (!workspace || workspace_bytes < need || !izb_aligned(workspace, 16))) return IZB_ERR_BAD_ARG;
     p.prefix.chunk = pl.prefix_chunk;
@@ -737,7 +823,10 @@ int32_t izb_shared_prefix_decode_gqa_attention(izb_ctx* ctx, izb_stream stream, 
     p.kv_heads = kv_heads;
     p.g = heads / kv_heads;
     p.row_blocks = pl.row_blocks;
-    p.scale_log2 = scale * LOG2E;
+    p.status = ctx->d_status;
+    p.q_sign = scale < 0.f ? 0x80008000u : 0u;
+    p.scale_log2 = fmaxf(fabsf(scale) * LOG2E, 1e-30f);  // not 0: a masked product is -inf and must stay it
+    p.margin = 8.f / p.scale_log2;
     const int64_t prefix_items = groups * pl.prefix_chunks * kv_heads * pl.row_blocks, items = prefix_items + batch * kv_heads * pl.own_chunks;
     if (items > INT32_MAX) return IZB_ERR_UNSUPPORTED;
     p.prefix_items = static_cast<int>(prefix_items);

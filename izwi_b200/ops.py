@@ -4,6 +4,7 @@ libizwi_b200.so; none has a PyTorch or CPU fallback."""
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -231,9 +232,15 @@ def sample_rows(logits: torch.Tensor, temperature: float, top_k: int, top_p: flo
     return idx.reshape(logits.shape[:-1])
 
 
-def _stream_of(t: torch.Tensor) -> C.c_void_p:
-    """The current stream of the tensor's device, whichever device is current."""
-    return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+# The current stream of a device, whichever device is current.  The raw getter: building a torch.cuda.Stream costs a
+# microsecond a call, which counts in steps that are made of few small launches.
+_stream_of_device = torch._C._cuda_getCurrentRawStream
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(entry: str, *args) -> int:
+    """A workspace query of the library: a pure function of its arguments (the context handle among them)."""
+    return getattr(L.lib(), entry)(*args)
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: int | None = None, finished: torch.Tensor | None = None,
@@ -245,32 +252,35 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: int | None = 
     if scores.dim() != 2 or scores.dtype != torch.float32 or not scores.is_contiguous():
         raise ValueError("beam_select: scores must be contiguous fp32 [groups, beams]")
     groups, beams = scores.shape
-    x = logits.reshape(-1, logits.shape[-1])
-    if x.dtype not in DTYPE or not x.is_cuda or x.stride(1) != 1 or x.shape[0] != groups * beams:
+    x = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
+    rows, vocab = x.shape
+    code, dev = DTYPE.get(x.dtype), x.device
+    if code is None or not x.is_cuda or x.stride(1) != 1 or rows != groups * beams:
         raise ValueError("beam_select: logits must be bf16 / fp32 / fp16 CUDA rows, one for each beam")
     if finished is not None and (finished.shape != scores.shape or finished.dtype != torch.uint8 or not finished.is_contiguous()):
         raise ValueError("beam_select: finished must be contiguous uint8 [groups, beams]")
-    dev = x.device
     if scores.device != dev or (finished is not None and finished.device != dev):
         raise ValueError("beam_select: tensors on different devices")
     n = beams if n_out is None else int(n_out)
+    ctx = Context.get(dev.index)
+    need = _workspace_bytes("izb_beam_select_workspace_bytes", ctx.handle.value, code, groups, beams, vocab, n)
     if out is None:
-        ints = torch.empty(2, groups, max(n, 0), device=dev, dtype=torch.int32)
-        out = (torch.empty(groups, max(n, 0), device=dev, dtype=torch.float32), ints[0], ints[1],
-               torch.empty(groups, max(n, 0), device=dev, dtype=torch.uint8))
+        if n == beams and finished is not None:  # the cheapest allocations there are
+            out = (torch.empty_like(scores), torch.empty_like(scores, dtype=torch.int32), torch.empty_like(scores, dtype=torch.int32),
+                   torch.empty_like(finished))
+        else:
+            shape = (groups, max(n, 0))
+            out = (torch.empty(shape, device=dev, dtype=torch.float32), torch.empty(shape, device=dev, dtype=torch.int32),
+                   torch.empty(shape, device=dev, dtype=torch.int32), torch.empty(shape, device=dev, dtype=torch.uint8))
     else:
         for t, d in zip(out, (torch.float32, torch.int32, torch.int32, torch.uint8)):
             if t is not None and (t.shape != (groups, n) or t.dtype != d or t.device != dev or not t.is_contiguous()):
                 raise ValueError("beam_select: out must be contiguous [groups, n_out] fp32, int32, int32, uint8")
-    ctx = Context.get(dev.index)
-    lib = L.lib()
-    code, vocab = DTYPE[x.dtype], x.shape[1]
-    need = lib.izb_beam_select_workspace_bytes(ctx.handle, code, groups, beams, vocab, n)
-    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
-    L.check(lib.izb_beam_select(ctx.handle, _stream_of(x), x.data_ptr(), code, groups, beams, vocab, x.stride(0) if groups * beams > 1 else vocab,
-                                scores.data_ptr(), None if finished is None else finished.data_ptr(), int(eos), n, out[0].data_ptr(),
-                                out[1].data_ptr(), out[2].data_ptr(), None if out[3] is None else out[3].data_ptr(), _ptr(ws), need),
-            "izb_beam_select")
+    ws = torch.empty(need, device=dev, dtype=torch.uint8)
+    L.check(L.lib().izb_beam_select(ctx.handle, _stream_of_device(dev.index), x.data_ptr(), code, groups, beams, vocab,
+                                    x.stride(0) if rows > 1 else vocab, scores.data_ptr(), None if finished is None else finished.data_ptr(),
+                                    int(eos), n, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
+                                    None if out[3] is None else out[3].data_ptr(), ws.data_ptr(), need), "izb_beam_select")
     return tuple(out)
 
 
@@ -286,7 +296,7 @@ def beam_trace(parents: torch.Tensor, tokens: torch.Tensor, last: torch.Tensor) 
     picks = last.shape[1]
     out = torch.empty(groups, picks, steps, device=parents.device, dtype=torch.int32)
     ctx = Context.get(parents.device.index)
-    L.check(L.lib().izb_beam_trace(ctx.handle, _stream_of(parents), parents.data_ptr(), tokens.data_ptr(), steps, groups, beams,
+    L.check(L.lib().izb_beam_trace(ctx.handle, _stream_of_device(parents.device.index), parents.data_ptr(), tokens.data_ptr(), steps, groups, beams,
                                    last.data_ptr(), picks, out.data_ptr(), steps), "izb_beam_trace")
     return out
 

@@ -9,7 +9,7 @@ import ctypes as C
 import torch
 
 from . import _lib as L
-from .ops import Context, _ptr, _stream, _stream_of
+from .ops import Context, _ptr, _stream, _stream_of_device, _workspace_bytes
 
 DEFAULT_KV_PAGE_SIZE = 64                     # paged.rs:10
 QUANT = {"none": 0, "int8": 1, "q4_0": 2}
@@ -128,31 +128,35 @@ def shared_prefix_attention(q: torch.Tensor, prefix: PagedKvCache, suffix: Paged
     Sequence i attends to the whole of prefix i // n and then to its own suffix.  The two bounds (default: what the
     tables hold) only size the split over the device."""
     b, h, d = q.shape
-    if q.dtype != torch.bfloat16 or not q.is_cuda or q.stride(2) != 1 or q.stride(1) != d:
+    dev, groups, kvh = q.device, prefix.batch, prefix.kv_heads
+    q_row, q_head, q_one = q.stride()
+    if q.dtype != torch.bfloat16 or not q.is_cuda or q_one != 1 or q_head != d:
         raise ValueError("shared_prefix_attention: q must be bf16 [sequences, heads, head_dim] with dense heads")
-    groups = prefix.batch
-    if groups == 0 or b % groups != 0 or d != prefix.head_dim or h % prefix.kv_heads != 0:
-        raise ValueError(f"shared_prefix_attention: q {tuple(q.shape)} does not fit {groups} prefixes of {prefix.kv_heads} x {prefix.head_dim}")
-    if suffix is not None and (suffix.batch != b or suffix.kv_heads != prefix.kv_heads or suffix.head_dim != d):
+    if groups == 0 or b % groups != 0 or d != prefix.head_dim or h % kvh != 0:
+        raise ValueError(f"shared_prefix_attention: q {tuple(q.shape)} does not fit {groups} prefixes of {kvh} x {prefix.head_dim}")
+    if suffix is not None and (suffix.batch != b or suffix.kv_heads != kvh or suffix.head_dim != d):
         raise ValueError("shared_prefix_attention: the suffix must hold one sequence per query, with the prefix's heads")
-    if prefix.page_table.device != q.device or (suffix is not None and suffix.page_table.device != q.device):
+    if prefix.page_table.device != dev or (suffix is not None and suffix.page_table.device != dev):
         raise ValueError("shared_prefix_attention: tensors on different devices")
     if out is None:
-        out = torch.empty(b, h, d, device=q.device, dtype=torch.bfloat16)
-    elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != q.device or out.stride(2) != 1 or out.stride(1) != d:
-        raise ValueError("shared_prefix_attention: out must be like q")
+        out, out_row = torch.empty((b, h, d), device=dev, dtype=torch.bfloat16), h * d
+    else:
+        out_row = out.stride(0)
+        if out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != dev or out.stride(2) != 1 or out.stride(1) != d:
+            raise ValueError("shared_prefix_attention: out must be like q")
     if b == 0:
         return out
+    if b == 1:
+        q_row = out_row = h * d
     most_p = prefix.max_tokens if max_prefix_len is None else int(max_prefix_len)
     most_s = 0 if suffix is None else suffix.max_tokens if max_seq_len is None else int(max_seq_len)
-    ctx, lib = Context.get(q.device.index), L.lib()
-    need = lib.izb_shared_prefix_decode_gqa_attention_workspace_bytes(ctx.handle, groups, b // groups, h, prefix.kv_heads, d, most_p, most_s)
-    ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
-    L.check(lib.izb_shared_prefix_decode_gqa_attention(
-        ctx.handle, _stream_of(q), q.data_ptr(), C.byref(prefix._desc), prefix.seq_lens.data_ptr(),
-        None if suffix is None else C.byref(suffix._desc), None if suffix is None else suffix.seq_lens.data_ptr(), out.data_ptr(), groups,
-        b // groups, h, most_p, most_s, q.stride(0) if b > 1 else h * d, out.stride(0) if b > 1 else h * d, float(d ** -0.5 if scale is None else scale), _ptr(ws), need),
-        "izb_shared_prefix_decode_gqa_attention")
+    ctx = Context.get(dev.index)
+    need = _workspace_bytes("izb_shared_prefix_decode_gqa_attention_workspace_bytes", ctx.handle.value, groups, b // groups, h, kvh, d, most_p, most_s)
+    ws = torch.empty(need, device=dev, dtype=torch.uint8)
+    L.check(L.lib().izb_shared_prefix_decode_gqa_attention(
+        ctx.handle, _stream_of_device(dev.index), q.data_ptr(), prefix._desc, prefix.seq_lens.data_ptr(), None if suffix is None else suffix._desc,
+        None if suffix is None else suffix.seq_lens.data_ptr(), out.data_ptr(), groups, b // groups, h, most_p, most_s, q_row, out_row,
+        d ** -0.5 if scale is None else scale, ws.data_ptr(), need), "izb_shared_prefix_decode_gqa_attention")
     return out
 
 
@@ -193,7 +197,7 @@ class PagedLayers:
         elif out.shape != table.shape or out.dtype != torch.int32 or not out.is_contiguous() or out.device != table.device:
             raise ValueError("reorder: out must be like the page table")
         ctx = Context.get(table.device.index)
-        L.check(L.lib().izb_kv_pages_reorder(ctx.handle, _stream_of(table), self._array, len(self.caches), parents.data_ptr(), parents.shape[0],
+        L.check(L.lib().izb_kv_pages_reorder(ctx.handle, _stream_of_device(table.device.index), self._array, len(self.caches), parents.data_ptr(), parents.shape[0],
                                              parents.shape[1], self.caches[0].seq_lens.data_ptr(), out.data_ptr()), "izb_kv_pages_reorder")
         return out
 
