@@ -555,103 +555,134 @@ __global__ void __launch_bounds__(RO_THREADS) kv_pages_reorder_kernel(const __gr
 //
 // A walk is a chain of dependent reads, one per step (0.25 us each from memory: 1,027 us for 4096 steps).  Up to 32
 // beams, `beams` lanes hold a step's parents, so a step of the walk is a shuffle among them; and the steps are cut into
-// chunks, 32 / beams of them side by side in a warp: first every chunk maps all beams at its end to beams at its
-// start, then the maps are chained, and then every chunk is walked again from where the walks enter it, writing tokens.
+// chunks, 32 / beams of them side by side in a warp, one warp after the other: first every chunk maps all beams at its
+// end to beams at its start and a warp's chunks are chained into one map, then the warps' maps are chained, and then
+// every chunk is walked again from where the walks enter it, writing tokens.
 constexpr int TR_WARPS = 32;
-constexpr int TR_MAX_CHUNKS = 512;
 constexpr int TR_AHEAD = 16;    // steps whose rows a lane has in flight
 constexpr int TR_NONE = 0xFF;   // a walk that has left [0, beams)
+
+// Rows s0 .. s0 + 15 of a lane's column (those below n), `ld` apart; s0 + 16 <= n for every lane of the warp: no tests.
+__device__ __forceinline__ void trace_rows(int (&r)[TR_AHEAD], const int* from, long long ld, int s0, int n, bool whole) {
+    const int* at = from + s0 * ld;
+    if (whole) {
+#pragma unroll
+        for (int j = 0; j < TR_AHEAD; ++j, at += ld) r[j] = __ldg(at);
+    } else {
+#pragma unroll
+        for (int j = 0; j < TR_AHEAD; ++j, at += ld) r[j] = s0 + j < n ? __ldg(at) : 0;
+    }
+}
 
 __global__ void __launch_bounds__(TR_WARPS * 32)
     beam_trace_chunks_kernel(const int* __restrict__ parents, const int* __restrict__ tokens, const int* __restrict__ last,
                              int* __restrict__ out, int steps, int beams, int picks, long long groups, long long ld_out, int chunk,
-                             int* status) {
+                             int ranks, int* status) {
     izb::pdl_launch_dependents();
     izb::pdl_wait();
-    __shared__ uint8_t map[TR_MAX_CHUNKS][32];    // beam at the chunk's end -> beam at the end of the chunk before
-    __shared__ uint8_t enter[TR_MAX_CHUNKS][32];  // where each of `beams` walks enters the chunk
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long group = blockIdx.x;
+    // in the first CTA of a group: beam at the end of a warp's steps -> beam at the end of the warp's before
+    __shared__ int map[TR_WARPS][32];
+    // where each of `beams` walks enters a warp's steps
+    __shared__ int enter[TR_WARPS][32];
+    const int lane = threadIdx.x & 31, here = threadIdx.x >> 5, rank = static_cast<int>(blockIdx.x) % ranks;
+    const int per_cta = static_cast<int>(blockDim.x >> 5), warp = rank * per_cta + here;
+    const long long group = blockIdx.x / ranks, ld = groups * beams;
+    auto sync_group = [&]() {
+        if (ranks > 1) izb::cluster_sync_all();
+        else __syncthreads();
+    };
     const int chunks = (steps + chunk - 1) / chunk;
     const int side = 32 / beams, sub = lane / beams, me = lane - sub * beams, base = sub * beams;
-    const long long ld = groups * beams;
+    const int c = warp * side + sub;
+    const long long lo = static_cast<long long>(c) * chunk;
+    const int n = sub < side && c < chunks ? static_cast<int>(steps - lo < chunk ? steps - lo : chunk) : 0;  // steps of this lane's chunk
+    const int warps = (chunks + side - 1) / side;                    // that have steps
+    const int most = __reduce_max_sync(0xFFFFFFFFu, n);
+    const bool even = __all_sync(0xFFFFFFFFu, n == most || sub >= side);
+    const int* par = parents + (n ? lo : 0) * ld + group * beams + me;
+    const int* tok = tokens + (n ? lo : 0) * ld + group * beams + me;
     // rows of out on 16-byte boundaries take four tokens a store: a lane writes a row of its own, so every store touches
-    // as many sectors as it has lanes (4096 steps, 32 x 8 walks: 38.8 us with single stores)
-    const bool wide = ld_out % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-    const int* par = parents + group * beams + me;
-    const int* tok = tokens + group * beams + me;
-    // `at` one step back; to: what shuffle brought from the lane of beam `at`
+    // as many sectors as it has lanes (4096 steps, 32 x 8 walks: 38.8 us with single stores, 26.6 us with these)
+    const bool wide = ld_out % 4 == 0 && chunk % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+    // `at` one step back; to: what the shuffle brought from the lane of beam `at`
     auto back = [&](int at, int to) { return at == TR_NONE || static_cast<unsigned>(to) >= static_cast<unsigned>(beams) ? TR_NONE : to; };
 
-    for (int c0 = warp * side; c0 < chunks; c0 += TR_WARPS * side) {
-        const int c = c0 + sub, lo = c * chunk;
-        const int n = sub < side && c < chunks ? min(steps - lo, chunk) : 0;  // steps of this lane's chunk
-        const int most = min(steps - c0 * chunk, chunk);                       // the first chunk of a warp is never shorter
-        int at = me;
+    // steps that fit one read are read once, tokens and the walks' ends with them: a short trace waits for memory once
+    const bool once = most <= TR_AHEAD;
+    int r[TR_AHEAD], t[TR_AHEAD];
+    if (once) {
+        trace_rows(r, par, ld, 0, n, even && n == TR_AHEAD);
+        trace_rows(t, tok, ld, 0, n, even && n == TR_AHEAD);
+    }
+    int end = warp == 0 && lane < beams && lane < picks ? last[group * picks + lane] : -1;
+
+    int mine = me;  // beam `me` at the end of this lane's chunk -> beam at its start
+    if (chunks > 1 && (side > 1 || warp > 0)) {  // nothing leads on from the first chunk of all
         for (int s0 = (most - 1) / TR_AHEAD * TR_AHEAD; s0 >= 0; s0 -= TR_AHEAD) {
-            int r[TR_AHEAD];
-#pragma unroll
-            for (int j = 0; j < TR_AHEAD; ++j) r[j] = s0 + j < n ? par[(lo + s0 + j) * ld] : 0;
+            if (!once) trace_rows(r, par, ld, s0, n, even && n && s0 + TR_AHEAD <= most);
 #pragma unroll
             for (int j = TR_AHEAD - 1; j >= 0; --j) {
-                const int to = __shfl_sync(0xFFFFFFFFu, r[j], (base + at) & 31);
-                if (s0 + j < n) at = back(at, to);
+                const int to = __shfl_sync(0xFFFFFFFFu, r[j], (base + mine) & 31);
+                if (s0 + j < n) mine = back(mine, to);
             }
         }
-        if (n) map[c][me] = static_cast<uint8_t>(at);
+    }
+    if (n == 0) mine = me;  // a chunk past the end leads nowhere else
+    {
+        int at = lane < beams ? lane : TR_NONE;
+        for (int k = side - 1; k >= 0; --k) {
+            const int to = __shfl_sync(0xFFFFFFFFu, mine, (k * beams + at) & 31);
+            at = at == TR_NONE ? TR_NONE : to;
+        }
+        if (ranks > 1) izb::st_cluster_f32(izb::cluster_map_shared(izb::smem_u32(&map[warp][lane]), 0), __int_as_float(at));
+        else map[warp][lane] = at;
     }
     for (int p0 = 0; p0 < picks; p0 += beams) {
-        __syncthreads();
+        sync_group();
         if (warp == 0) {
-            int at = TR_NONE;
-            if (lane < beams && p0 + lane < picks) {
-                const int b = last[group * picks + p0 + lane];
-                if (b >= 0 && b < beams) at = b;
-            }
-            for (int c = chunks - 1; c >= 0; --c) {
-                enter[c][lane] = static_cast<uint8_t>(at);
-                at = at == TR_NONE ? TR_NONE : map[c][at];
+            if (p0 > 0) end = lane < beams && p0 + lane < picks ? last[group * picks + p0 + lane] : -1;
+            int at = end >= 0 && end < beams ? end : TR_NONE;
+            for (int w = warps - 1; w >= 0; --w) {
+                if (ranks > 1) izb::st_cluster_f32(izb::cluster_map_shared(izb::smem_u32(&enter[w][lane]), w / per_cta), __int_as_float(at));
+                else enter[w][lane] = at;
+                at = at == TR_NONE ? TR_NONE : map[w][at];
             }
         }
-        __syncthreads();
+        sync_group();
+        if (warp >= warps) continue;
         const bool walks = p0 + me < picks;
-        int* dst = out + (group * picks + p0 + (walks ? me : 0)) * ld_out;
-        for (int c0 = warp * side; c0 < chunks; c0 += TR_WARPS * side) {
-            const int c = c0 + sub, lo = c * chunk;
-            const int n = sub < side && c < chunks ? min(steps - lo, chunk) : 0;
-            const int most = min(steps - c0 * chunk, chunk);
-            int at = n ? enter[c][me] : TR_NONE;
-            bool lost = false;
-            for (int s0 = (most - 1) / TR_AHEAD * TR_AHEAD; s0 >= 0; s0 -= TR_AHEAD) {
-                int r[TR_AHEAD], t[TR_AHEAD];
+        int* dst = out + (group * picks + p0 + (walks ? me : 0)) * ld_out + (n ? lo : 0);
+        // from the warp's end through the chunks behind this lane's own
+        int at = enter[warp][me];
+        for (int k = side - 1; k > 0; --k) {
+            const int to = __shfl_sync(0xFFFFFFFFu, mine, (k * beams + at) & 31);
+            if (k > sub && at != TR_NONE) at = to;
+        }
+        bool lost = false;
+        for (int s0 = (most - 1) / TR_AHEAD * TR_AHEAD; s0 >= 0; s0 -= TR_AHEAD) {
+            const bool whole = even && n && s0 + TR_AHEAD <= most;
+            if (!once) trace_rows(r, par, ld, s0, n, whole);
+            if (!once || p0 > 0) trace_rows(t, tok, ld, s0, n, whole);  // the tokens' registers become the results
 #pragma unroll
-                for (int j = 0; j < TR_AHEAD; ++j) {
-                    const bool ok = s0 + j < n;
-                    r[j] = ok ? par[(lo + s0 + j) * ld] : 0;
-                    t[j] = ok ? tok[(lo + s0 + j) * ld] : 0;
-                }
-#pragma unroll
-                for (int j = TR_AHEAD - 1; j >= 0; --j) {
-                    const int from = (base + at) & 31;
-                    const int token = __shfl_sync(0xFFFFFFFFu, t[j], from), to = __shfl_sync(0xFFFFFFFFu, r[j], from);
-                    t[j] = at == TR_NONE ? -1 : token;
-                    if (s0 + j < n) {
-                        lost |= at == TR_NONE;
-                        at = back(at, to);
-                    }
-                }
-                if (walks && wide && s0 + TR_AHEAD <= n) {
-#pragma unroll
-                    for (int j = 0; j < TR_AHEAD; j += 4)
-                        *reinterpret_cast<int4*>(dst + lo + s0 + j) = make_int4(t[j], t[j + 1], t[j + 2], t[j + 3]);
-                } else if (walks) {
-#pragma unroll
-                    for (int j = 0; j < TR_AHEAD; ++j)
-                        if (s0 + j < n) dst[lo + s0 + j] = t[j];
+            for (int j = TR_AHEAD - 1; j >= 0; --j) {
+                const int from = (base + at) & 31;
+                const int token = __shfl_sync(0xFFFFFFFFu, t[j], from), to = __shfl_sync(0xFFFFFFFFu, r[j], from);
+                t[j] = at == TR_NONE ? -1 : token;
+                if (s0 + j < n) {
+                    lost |= at == TR_NONE;
+                    at = back(at, to);
                 }
             }
-            if (walks && lost) atomicExch(status, 9);
+            if (walks && wide && s0 + TR_AHEAD <= n) {
+#pragma unroll
+                for (int j = 0; j < TR_AHEAD; j += 4) *reinterpret_cast<int4*>(dst + s0 + j) = make_int4(t[j], t[j + 1], t[j + 2], t[j + 3]);
+            } else if (walks) {
+#pragma unroll
+                for (int j = 0; j < TR_AHEAD; ++j)
+                    if (s0 + j < n) dst[s0 + j] = t[j];
+            }
         }
+        if (walks && lost) atomicExch(status, 9);
     }
 }
 
@@ -804,11 +835,13 @@ int32_t izb_beam_trace(izb_ctx* ctx, izb_stream stream, const int32_t* parents, 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (beams <= 32) {
         // one chunk for every place of the CTA's warps, of whole reads ahead
-        const int64_t places = TR_WARPS * (32 / beams), fit = places < TR_MAX_CHUNKS ? places : TR_MAX_CHUNKS;
-        const int64_t chunk = ((steps + fit - 1) / fit + TR_AHEAD - 1) / TR_AHEAD * TR_AHEAD;
-        IZB_CUDA_TRY(izb::launch_chained(ctx, beam_trace_chunks_kernel, dim3(static_cast<unsigned>(groups)), dim3(TR_WARPS * 32), 0, st, parents,
-                                         tokens, last, out, static_cast<int>(steps), beams, picks, static_cast<long long>(groups),
-                                         static_cast<long long>(ld_out), static_cast<int>(chunk), ctx->d_status + 6));
+        const int64_t places = TR_WARPS * (32 / beams), chunk = ((steps + places - 1) / places + TR_AHEAD - 1) / TR_AHEAD * TR_AHEAD;
+        const int64_t warps = ((steps + chunk - 1) / chunk + 32 / beams - 1) / (32 / beams);  // a short trace is one warp's
+        const int ranks = warps >= 8 && groups <= ctx->sm_count ? 4 : 1;
+        IZB_CUDA_TRY(izb::launch_chained_cluster(ctx, ranks, beam_trace_chunks_kernel, dim3(static_cast<unsigned>(groups * ranks)),
+                                                 dim3(static_cast<unsigned>((warps + ranks - 1) / ranks * 32)), 0, st, parents, tokens, last, out, static_cast<int>(steps), beams, picks,
+                                                 static_cast<long long>(groups), static_cast<long long>(ld_out), static_cast<int>(chunk), ranks,
+                                                 ctx->d_status + 6));
     } else {
         const unsigned grid = static_cast<unsigned>((groups * picks + 127) / 128);
         IZB_CUDA_TRY(izb::launch_chained(ctx, beam_trace_kernel, dim3(grid), dim3(128), 0, st, parents, tokens, last, out,
