@@ -8,16 +8,19 @@
 // once and its 16-bit fragments are used by S * G rows on the tensor cores.
 //
 // Work: an item is (group, KV head, block of query rows, chunk of prefix tokens) or (sequence, KV head, chunk of its
-// own tokens); all items go out in one launch, one CTA each.  A CTA walks its chunk in tiles with a running maximum
-// and sum per row and leaves (max, sum, weighted values) for a second launch that joins the chunks
+// own tokens); all items go out in one launch, one CTA each, or, with many rows or a long prefix, those of the prefix in
+// a launch of their own on tensor memory (shared_prefix_tc.cu).  A CTA walks its chunk in tiles with a running maximum
+// and sum per row and leaves (max, sum, weighted values) for a last launch that joins the chunks
 // of every (sequence, head).  fp32 for scores, maxima, sums and accumulators; p is rounded to bf16 for the product
 // with v (half a step: 2^-9 relative, independent per token, which is what the bf16 output itself carries).
 #include <climits>
 #include <cmath>
 
-#include "izb_common.cuh"
+#include "shared_prefix.cuh"
 
 namespace {
+
+using namespace izb::shared_prefix;
 
 constexpr int SP_THREADS = 256;      // four computing warps, four that copy
 constexpr int SP_TILE = 128;         // chunks are multiples of this, and so of every tile size
@@ -25,41 +28,6 @@ constexpr int SP_MAX_CHUNK = 768;    // tokens per item: with their table of pla
 constexpr int SP_MAX_G = 16;         // query heads per KV head: the rows of one own-pages item
 constexpr float LOG2E = 1.4426950408889634f;
 
-struct Source {
-    const uint8_t* k;
-    const uint8_t* v;
-    const float* k_scales;
-    const float* v_scales;
-    const int* table;
-    const int* lens;
-    long long max_pages;
-    int quant, page_size;
-    int max_len;     // lengths on the device are cut to this
-    int chunk;       // tokens per item
-    int n_chunks;
-};
-
-struct Params {
-    Source prefix, own;
-    const __nv_bfloat16* q;
-    float* acc;       // [rows][chunks][D], rows = batch * heads
-    float2* ml;       // [rows][chunks]: maximum (log2 scale) and sum
-    long long ld_q;
-    int seqs, heads, kv_heads, g;  // sequences per group, query heads per KV head
-    int row_blocks, prefix_items;
-    int* status;
-    uint32_t q_sign;   // flips q where the scale is negative, so that the largest product is the largest score
-    float scale_log2;  // |scale| / ln 2
-    float margin;      // 8 / scale_log2: a growth of 2^8 in weight, in units of the products
-};
-
-// `n` of the 16 (4) bytes come from src, the rest is zero
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int n) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, int n) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
@@ -69,39 +37,7 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 __device__ __forceinline__ float lds_f32(uint32_t addr) { return __uint_as_float(izb::lds32(addr)); }
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t r;
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-    return r;
-}
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
-// Two Int8 codes in the low bytes of the halves of x (code = byte - 128) -> bf16x2.  128 + (byte & 127) is the bf16
-// 0x4300 | low bits; what is left to add is -256 for bytes below 128 and -128 above: every step is exact.
-__device__ __forceinline__ uint32_t int8_pair(uint32_t x) {
-    return hfma2((x & 0x007F007Fu) | 0x43004300u, 0x3F803F80u, (~x & 0x00800080u) | 0xC300C300u);
-}
-// Two 4-bit codes in the low nibbles of the halves (code = nibble - 8) -> bf16x2, exact.
-__device__ __forceinline__ uint32_t q4_pair(uint32_t x) { return hfma2((x & 0x000F000Fu) | 0x43004300u, 0x3F803F80u, 0xC308C308u); }
-// code * scale rounded to bf16 as the stored value is defined.  The fp32 scale enters as two bf16 parts; the product
-// with the small part is rounded to 8 bits at 2^-8 of the value, so the sum's one rounding sees the product to 2^-17.
-__device__ __forceinline__ uint32_t q4_value(uint32_t code2, uint32_t hi2, uint32_t lo2) { return hfma2(code2, hi2, hmul2(code2, lo2)); }
-__device__ __forceinline__ void split_scale(float s, uint32_t& hi2, uint32_t& lo2) {
-    const __nv_bfloat16 h = __float2bfloat16_rn(s);
-    const __nv_bfloat16 l = __float2bfloat16_rn(s - __bfloat162float(h));
-    const uint32_t hu = __bfloat16_as_ushort(h), lu = __bfloat16_as_ushort(l);
-    hi2 = hu | (hu << 16);
-    lo2 = lu | (lu << 16);
-}
+__device__ __forceinline__ void split_scale(float s, uint32_t& hi2, uint32_t& lo2) { split_scales(s, s, hi2, lo2); }
 
 // How a tile of one item lies in shared memory.  Four computing warps share a tile, WT tokens each.
 template <int D, int Q>
@@ -258,6 +194,7 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<D, MT_LAUNCH>::COMPUTE));
     float o[MT][DT][4], m[MT][2], l[MT][2];
     {
+        const CodeBits<Q> bits;
         uint32_t qa[Q_IN_REGS ? MT : 1][Q_IN_REGS ? KS : 1][4];
         // fragment of query rows 16 mt.. for product step ks.  bf16: channels in order (ldmatrix); codes: the order of d
         // inside a product is free as long as both operands use it, lane tq takes the D / 4 channels from tq * D / 4, four
@@ -334,8 +271,8 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
                                     const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                                     for (int i = 0; i < 4; ++i) {
-                                        b[n][h * 8 + i * 2] = hmul2(int8_pair(izb::prmt(x[i], 0u, 0x4140)), sc2);
-                                        b[n][h * 8 + i * 2 + 1] = hmul2(int8_pair(izb::prmt(x[i], 0u, 0x4342)), sc2);
+                                        b[n][h * 8 + i * 2] = hmul2(bits.pair(izb::prmt(x[i], 0u, 0x4140)), sc2);
+                                        b[n][h * 8 + i * 2 + 1] = hmul2(bits.pair(izb::prmt(x[i], 0u, 0x4342)), sc2);
                                     }
                                 }
                             } else {
@@ -352,7 +289,7 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
 #pragma unroll
                                 for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-                                    for (int e = 0; e < 4; ++e) b[n][i * 4 + e] = q4_value(q4_pair(x[i] >> (4 * e)), hi2, lo2);
+                                    for (int e = 0; e < 4; ++e) b[n][i * 4 + e] = q4_value(bits.pair(x[i] >> (4 * e)), hi2, lo2);
                             }
                         }
 #pragma unroll
@@ -465,9 +402,9 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
 #pragma unroll
                             for (int j = 0; j < DT; ++j) {
                                 const int w = j >> 2, by = j & 3;
-                                const uint32_t sel = by | ((4 + by) << 8);  // byte `by` of both words; int8_pair masks the rest
-                                accumulate(j, hmul2(int8_pair(izb::prmt(x[0][w], x[1][w], sel)), s01),
-                                           hmul2(int8_pair(izb::prmt(x[2][w], x[3][w], sel)), s23));
+                                const uint32_t sel = by | ((4 + by) << 8);  // byte `by` of both words; the pair's mask drops the rest
+                                accumulate(j, hmul2(bits.pair(izb::prmt(x[0][w], x[1][w], sel)), s01),
+                                           hmul2(bits.pair(izb::prmt(x[2][w], x[3][w], sel)), s23));
                             }
                         } else {
                             const int blk = gq * (D / 8) / 32;
@@ -493,7 +430,7 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
                             for (int j = 0; j < DT; ++j) {
                                 const uint32_t sel = (j & 4) ? 0x7632u : 0x5410u;  // four codes of both tokens side by side
                                 const uint32_t w01 = izb::prmt(x[0][j >> 3], x[1][j >> 3], sel), w23 = izb::prmt(x[2][j >> 3], x[3][j >> 3], sel);
-                                accumulate(j, q4_value(q4_pair(w01 >> (4 * (j & 3))), h01, l01), q4_value(q4_pair(w23 >> (4 * (j & 3))), h23, l23));
+                                accumulate(j, q4_value(bits.pair(w01 >> (4 * (j & 3))), h01, l01), q4_value(bits.pair(w23 >> (4 * (j & 3))), h23, l23));
                             }
                         }
                     }
@@ -564,8 +501,6 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
         *reinterpret_cast<float4*>(p.acc + slot_of(r) * D + d) = a;
     }
 }
-
-__device__ __forceinline__ int length_of(const Source& s, int row) { return min(max(s.lens[row], 0), s.max_len); }
 
 template <int D, int MT>
 __global__ void __launch_bounds__(SP_THREADS, Regs<D, MT>::CTAS) shared_prefix_kernel(const __grid_constant__ Params p) {
@@ -660,43 +595,55 @@ __global__ void __launch_bounds__(128)
 
 // ---- host side ---------------------------------------------------------------------------------------------------
 struct Plan {
-    int rows;        // query rows of a prefix item: 16 or 32
+    bool tc;         // the prefix goes to the tensor-memory kernel
+    int rows;        // query rows of a prefix item
     int row_blocks;
     int prefix_chunk, prefix_chunks, own_chunk, own_chunks;
 };
 
 // Tokens per item.  `base` items per chunk of the sequence meet `slots` resident CTAs in waves; an item costs its
-// tiles plus about one tile for the query rows, the table of places and the result.  The split counts from the
-// fewest whose chunks fit the table of places are tried.
-int choose_chunk(int64_t base, int64_t tokens, int64_t slots) {
-    const int64_t tiles = (tokens + SP_TILE - 1) / SP_TILE;
-    const int64_t fewest = (tiles + SP_MAX_CHUNK / SP_TILE - 1) / (SP_MAX_CHUNK / SP_TILE), most = fewest + 48;
+// tiles plus `extra` for the query rows, the first loads and the result.  The split counts from the fewest whose chunks
+// are allowed are tried.
+int choose_chunk(int64_t base, int64_t tokens, int64_t slots, int tile, int extra, int most_tiles) {
+    const int64_t tiles = (tokens + tile - 1) / tile;
+    const int64_t fewest = (tiles + most_tiles - 1) / most_tiles, most = fewest + 63;
     int64_t best = 0, best_cost = INT64_MAX;
     for (int64_t n = fewest; n <= tiles && n <= most; ++n) {
         const int64_t per = (tiles + n - 1) / n, items = base * ((tiles + per - 1) / per);
-        const int64_t cost = ((items + slots - 1) / slots) * (per + 1);
+        const int64_t cost = ((items + slots - 1) / slots) * (per + extra);
         if (cost < best_cost) {
             best_cost = cost;
             best = per;
         }
         if (per == 1) break;
     }
-    return static_cast<int>(best * SP_TILE);
+    return static_cast<int>(best * tile);
 }
 
-Plan make_plan(const izb_ctx* ctx, int64_t groups, int64_t seqs, int kv_heads, int g, int head_dim, int64_t max_prefix, int64_t max_own) {
+Plan make_plan(const izb_ctx* ctx, int64_t groups, int64_t seqs, int kv_heads, int g, int head_dim, bool bf16, int64_t max_prefix, int64_t max_own) {
     Plan pl = {};
-    const int64_t rows = seqs * g;
-    const int64_t slots = (head_dim == 64 && rows <= 16 ? 3 : 2) * static_cast<int64_t>(ctx && ctx->sm_count > 0 ? ctx->sm_count : 148);
-    // the smallest block that holds the rows: a tile's fragments serve all rows of a block, idle rows cost mma steps
-    pl.rows = rows <= 16 ? 16 : 32;
+    const int64_t rows = seqs * g, sms = ctx && ctx->sm_count > 0 ? ctx->sm_count : 148;
+    // Which kernel takes the prefix.  Above 32 rows a second block of 32 would read the tiles again, and the tensor-memory
+    // kernel holds 128 or 256.  Up to 32 its rows are mostly idle, but a 128-token bf16 tile of D = 128 takes it 1,900
+    // cycles against 3,300 to 4,900 here; against that stand some 5 us for an item's first loads, tensor memory and result,
+    // so items have to be long (bf16, 32,768 tokens, 2 x 8 heads: 16 rows 53.8 us against 64.7, 32 rows 54.3 against 73.8;
+    // 12 tiles an item, 5 rows: 118 against 94).  Converting codes takes it 4,200 cycles a tile, which pays from 17 rows
+    // (Int8, 32,768 tokens, 2 x 8 heads, 32 rows: 73 against 85; at 8 tiles an item level, and then one launch for prefix
+    // and own pages is better than two); D = 64: 35 us against 18.5 at 12 tiles an item.
+    const int tc_rows = rows <= TC_ROWS ? TC_ROWS : 2 * TC_ROWS;
+    const int64_t tc_items = groups * kv_heads * ((rows + tc_rows - 1) / tc_rows);
+    const int tc_chunk = max_prefix > 0 ? choose_chunk(tc_items, max_prefix, sms, 128, 4, 1 << 20) : 0;
+    pl.tc = rows > 32 || (head_dim == 128 && (rows > 16 ? tc_chunk >= 12 * 128 : bf16 && tc_chunk >= 16 * 128));
+    pl.rows = pl.tc ? tc_rows : rows <= 16 ? 16 : 32;
     pl.row_blocks = static_cast<int>((rows + pl.rows - 1) / pl.rows);
+    const int64_t slots = (head_dim == 64 && (rows <= 16 || pl.tc) ? 3 : 2) * sms;  // of the other kernel
     if (max_prefix > 0) {
-        pl.prefix_chunk = choose_chunk(groups * kv_heads * pl.row_blocks, max_prefix, slots);
+        const int64_t base = groups * kv_heads * pl.row_blocks;
+        pl.prefix_chunk = pl.tc ? tc_chunk : choose_chunk(base, max_prefix, slots, SP_TILE, 1, SP_MAX_CHUNK / SP_TILE);
         pl.prefix_chunks = static_cast<int>((max_prefix + pl.prefix_chunk - 1) / pl.prefix_chunk);
     }
     if (max_own > 0) {
-        pl.own_chunk = choose_chunk(groups * seqs * kv_heads, max_own, slots);
+        pl.own_chunk = choose_chunk(groups * seqs * kv_heads, max_own, slots, SP_TILE, 1, SP_MAX_CHUNK / SP_TILE);
         pl.own_chunks = static_cast<int>((max_own + pl.own_chunk - 1) / pl.own_chunk);
     }
     return pl;
@@ -740,7 +687,7 @@ size_t smem_for(const Source& s) {
 
 template <int D, int MT>
 int launch_items(izb_ctx* ctx, cudaStream_t s, const Params& p, int64_t items) {
-    size_t smem = smem_for<D, MT>(p.prefix);
+    size_t smem = p.prefix_items > 0 ? smem_for<D, MT>(p.prefix) : 0;
     const size_t own = smem_for<D, 1>(p.own);
     if (own > smem) smem = own;
     auto kern = shared_prefix_kernel<D, MT>;
@@ -761,7 +708,11 @@ template <int D>
 int launch_dim(izb_ctx* ctx, cudaStream_t s, const Params& p, const Plan& pl, int64_t items, int64_t batch, __nv_bfloat16* out,
                long long ld_out) {
     if (items > 0) {
-        const int rc = pl.rows == 16 ? launch_items<D, 1>(ctx, s, p, items) : launch_items<D, 2>(ctx, s, p, items);
+        const int rc = pl.tc || pl.rows == 16 ? launch_items<D, 1>(ctx, s, p, items) : launch_items<D, 2>(ctx, s, p, items);
+        if (rc != IZB_OK) return rc;
+    }
+    if (pl.tc && p.prefix.n_chunks > 0) {
+        const int rc = launch_prefix_tc(ctx, s, p, D, batch / p.seqs);
         if (rc != IZB_OK) return rc;
     }
     IZB_CUDA_TRY(izb::launch_chained(ctx, shared_prefix_join_kernel<D>, dim3(static_cast<unsigned>(batch * p.heads)), dim3(128), 0, s, p, out,
@@ -780,8 +731,14 @@ size_t izb_shared_prefix_decode_gqa_attention_workspace_bytes(const izb_ctx* ctx
     if (groups <= 0 || seqs_per_group <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || head_dim <= 0 ||
         max_prefix_len < 0 || max_seq_len < 0 || groups > INT32_MAX / seqs_per_group || max_prefix_len > INT32_MAX || max_seq_len > INT32_MAX)
         return 0;
-    const Plan pl = make_plan(ctx, groups, seqs_per_group, kv_heads, heads / kv_heads, head_dim, max_prefix_len, max_seq_len);
-    return plan_bytes(pl, groups * seqs_per_group, heads, head_dim);
+    // the query does not know how the pages are stored: enough for either plan
+    size_t most = 0;
+    for (int bf16 = 0; bf16 < 2; ++bf16) {
+        const Plan pl = make_plan(ctx, groups, seqs_per_group, kv_heads, heads / kv_heads, head_dim, bf16 != 0, max_prefix_len, max_seq_len);
+        const size_t need = plan_bytes(pl, groups * seqs_per_group, heads, head_dim);
+        most = need > most ? need : most;
+    }
+    return most;
 }
 
 int32_t izb_shared_prefix_decode_gqa_attention(izb_ctx* ctx, izb_stream stream, const void* q, const izb_kv_pages* prefix,
@@ -807,7 +764,7 @@ int32_t izb_shared_prefix_decode_gqa_attention(izb_ctx* ctx, izb_stream stream, 
     if (ld_q < static_cast<int64_t>(heads) * d || ld_out < static_cast<int64_t>(heads) * d) return IZB_ERR_BAD_ARG;
     if (groups > INT32_MAX / seqs_per_group || groups * seqs_per_group > INT32_MAX / heads) return IZB_ERR_UNSUPPORTED;
     const int64_t batch = groups * seqs_per_group;
-    const Plan pl = make_plan(ctx, groups, seqs_per_group, kv_heads, heads / kv_heads, d, max_prefix_len, max_seq_len);
+    const Plan pl = make_plan(ctx, groups, seqs_per_group, kv_heads, heads / kv_heads, d, p.prefix.quant == IZB_KV_NONE, max_prefix_len, max_seq_len);
     const size_t need = plan_bytes(pl, batch, heads, d);
     if (need && (!workspace || workspace_bytes < need || !izb_aligned(workspace, 16))) return IZB_ERR_BAD_ARG;
     p.prefix.chunk = pl.prefix_chunk;
@@ -827,8 +784,8 @@ int32_t izb_shared_prefix_decode_gqa_attention(izb_ctx* ctx, izb_stream stream, 
     p.q_sign = scale < 0.f ? 0x80008000u : 0u;
     p.scale_log2 = fmaxf(fabsf(scale) * LOG2E, 1e-30f);  // not 0: a masked product is -inf and must stay it
     p.margin = 8.f / p.scale_log2;
-    const int64_t prefix_items = groups * pl.prefix_chunks * kv_heads * pl.row_blocks, items = prefix_items + batch * kv_heads * pl.own_chunks;
-    if (items > INT32_MAX) return IZB_ERR_UNSUPPORTED;
+    const int64_t prefix_items = pl.tc ? 0 : groups * pl.prefix_chunks * kv_heads * pl.row_blocks, items = prefix_items + batch * kv_heads * pl.own_chunks;
+    if (items > INT32_MAX || groups * pl.prefix_chunks > INT32_MAX / kv_heads / pl.row_blocks) return IZB_ERR_UNSUPPORTED;
     p.prefix_items = static_cast<int>(prefix_items);
     izb::DeviceGuard guard(ctx->device);
     if (!guard.ok) return IZB_ERR_LAUNCH;
