@@ -253,3 +253,69 @@ def test_agrees_with_paged_attention_over_copies_of_the_prompt(cuda):
     # each within half a step of the output and 2^-8 A of the exact result; A <= max |v|, here bounded by 1
     assert ((a - b).abs() <= 2 * HALF * a.abs() + 2 * HALF * 1.0).all()
     assert math.isfinite(float(a.sum()))
+
+
+@pytest.mark.parametrize("quant", ["none", "int8", "q4_0"])
+@pytest.mark.parametrize("seqs,heads,kvh,groups,length", [(8, 16, 4, 1, 60001), (12, 8, 4, 2, 29000), (4, 8, 4, 1, 80000)])
+def test_long_prefixes_of_few_rows(cuda, quant, seqs, heads, kvh, groups, length):
+    """Up to 32 rows over prefixes long enough for the tensor-memory kernel, the last chunk cut anywhere; the definition
+    computed on the GPU in 64 bits.  Pages of 24 tokens."""
+    from izwi_b200 import ops, paged
+    rng = np.random.default_rng(length)
+    d, page = 128, 24
+    lens = [length - 1000 * g for g in range(groups)]
+    prefix = Pool(rng, cuda, lens, kvh, d, page, quant, spare_pages=0)
+    q = torch.from_numpy(rng.normal(0, 2, (groups * seqs, heads, d)).astype(np.float32)).to(torch.bfloat16).to(cuda)
+    got = paged.shared_prefix_attention(q, prefix.cache, None).double()
+    ops.Context.get(0).check()
+    for g in range(groups):
+        k, v = (torch.from_numpy(x).to(cuda) for x in prefix.exact[g])
+        qd = q[g * seqs:(g + 1) * seqs].double().reshape(seqs, kvh, heads // kvh, d)
+        p = torch.softmax(torch.einsum("skgd,tkd->skgt", qd, k) * d ** -0.5, -1)
+        want = torch.einsum("skgt,tkd->skgd", p, v).reshape(seqs, heads, d)
+        a = torch.einsum("skgt,tkd->skgd", p, v.abs()).reshape(seqs, heads, d)
+        mag = (torch.einsum("skgd,tkd->skgt", qd.abs(), k.abs()).amax(-1) * d ** -0.5).reshape(seqs, heads, 1)
+        tol = HALF * want.abs() + a * (HALF + len(k) * 2.0 ** -24 + 2.0 ** -20 + torch.expm1(2 * mag * (d + 4) * 2.0 ** -24)) * (1 + HALF)
+        assert ((got[g * seqs:(g + 1) * seqs] - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("quant", ["none", "int8"])
+@pytest.mark.parametrize("page", [8, 5])
+def test_values_that_are_not_finite_behind_the_end(cuda, quant, page):
+    """Many rows (the tensor-memory kernel) over a length that ends inside a tile and a page; behind it lie NaN."""
+    rng = np.random.default_rng(page)
+    check(rng, cuda, 20, 8, Pool(rng, cuda, [133, 1, 127], 2, 64, page, quant), Pool(rng, cuda, [2] * 60, 2, 64, page, "none"))
+
+
+def test_two_graphs_share_a_workspace(cuda):
+    """Two captured calls with one workspace, replayed in turn: each leaves its own result."""
+    import ctypes as C
+
+    from izwi_b200 import _lib as L
+    from izwi_b200 import ops, paged  # noqa: F401
+    rng = np.random.default_rng(19)
+    lib, ctx = L.lib(), ops.Context.get(0)
+    sides = []
+    for plens, slens, seqs in (([500, 90], [9, 64, 0, 70], 2), ([2000], [30] * 20, 20)):
+        prefix, own = Pool(rng, cuda, plens, 2, 128, 64, "none"), Pool(rng, cuda, slens, 2, 128, 64, "none")
+        q = torch.from_numpy(rng.normal(0, 1, (len(slens), 8, 128)).astype(np.float32)).to(cuda).to(torch.bfloat16)
+        want = paged.shared_prefix_attention(q, prefix.cache, own.cache)
+        sides.append((prefix.cache, own.cache, q, seqs, want, torch.zeros_like(want)))
+    need = max(lib.izb_shared_prefix_decode_gqa_attention_workspace_bytes(ctx.handle, p.batch, n, 8, 2, 128, p.max_tokens, o.max_tokens)
+               for p, o, _, n, _, _ in sides)
+    ws = torch.empty(need, device=cuda, dtype=torch.uint8)
+    graphs = []
+    for p, o, q, n, _, out in sides:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            L.check(lib.izb_shared_prefix_decode_gqa_attention(
+                ctx.handle, C.c_void_p(torch.cuda.current_stream().cuda_stream), q.data_ptr(), C.byref(p._desc), p.seq_lens.data_ptr(),
+                C.byref(o._desc), o.seq_lens.data_ptr(), out.data_ptr(), p.batch, n, 8, p.max_tokens, o.max_tokens, 1024, 1024, 128 ** -0.5,
+                ws.data_ptr(), need), "capture")
+        graphs.append(graph)
+    for _ in range(3):
+        for graph in graphs:
+            graph.replay()
+    torch.cuda.synchronize()
+    for _, _, _, _, want, out in sides:
+        assert torch.equal(out, want)
