@@ -51,6 +51,9 @@ struct Layout {
     static constexpr int STAGE = 2 * (TILE_BYTES + SCALE_BYTES);
     // what two CTAs (D = 64: three) of an SM can hold
     static constexpr int STAGES = D == 128 ? (STAGE > 24 * 1024 ? 3 : 4) : STAGE > 24 * 1024 ? 2 : STAGE > 12 * 1024 ? 3 : 4;
+    // floats of a row of the final exchange between the warps: a store phase of bf16 tiles meets four rows of eight
+    // consecutive banks, of codes two rows of four 16-byte columns
+    static constexpr int EX_LD = Q == IZB_KV_NONE ? D + 8 : D + 4;
     // place of 16-byte chunk c of token row r: the chunk index is mixed with the row so that the eight lanes of a
     // shared-memory phase (ldmatrix: eight rows of one chunk; codes: two rows of four chunks) meet different banks
     static __device__ __forceinline__ int place(int r, int c) {
@@ -60,12 +63,11 @@ struct Layout {
     }
 };
 
-// shared memory of an item: query rows, table of token places, Int8 scales, then the tile ring, which the final
-// exchange between the warps reuses (rows of D + 4 floats: consecutive rows start four banks apart)
+// shared memory of an item: query rows, table of token places, Int8 scales, then the tile ring, which the exchange reuses
 template <int D, int MT, int Q>
 constexpr int item_smem(int chunk) {
     const int ring = Layout<D, Q>::STAGE * Layout<D, Q>::STAGES;
-    const int exchange = 4 * 16 * MT * (D + 4) * 4;
+    const int exchange = 4 * 16 * MT * Layout<D, Q>::EX_LD * 4;
     return 16 * MT * D * 2 + chunk * 4 + (Q == IZB_KV_INT8 ? chunk * 4 : 0) + (ring > exchange ? ring : exchange);
 }
 
@@ -81,12 +83,13 @@ struct Regs {
 
 struct ItemShared {
     unsigned long long full[4], empty[4];
+    long long slot[32];   // per row: its place among the partial results
     float2 wml[4][32];    // per warp and row: maximum and sum
     float factor[4][32];  // per warp and row: weight in the joined result
     int abort_flag;
 };
 
-// One item: n_rows (at most 16 MT) query rows from row0 that meet KV head kh of `src` row `src_row`, tokens [t0, t1).
+// One item: n_rows (at most 16 MT) query rows from row0 that meet KV head kh of `src` row `src_row`, a chunk of tokens from t0.
 // Warps 0..3 compute, each on its share of every tile with a maximum, sum and accumulator of its own; warps 4..7
 // copy tiles ahead of them through a ring of stages (cp.async onto an mbarrier), so that no warp waits for another one;
 // registers the copying warps do not need go to the computing ones (setmaxnreg; their shares add up to the launch's).
@@ -94,14 +97,12 @@ struct ItemShared {
 // for three quarters of its rows, while here a tile's fragments are read (or made from codes) exactly once.
 template <int D, int MT, int Q, int MT_LAUNCH>
 __device__ __forceinline__ void attend(const Params& p, const Source& src, int src_row, int kh, int seq0, int row0, int n_rows, int t0,
-                                       int t1, int chunk_slot, int chunks_total, uint8_t* smem, ItemShared& sh) {
+                                       int chunk_slot, int chunks_total, uint8_t* smem, ItemShared& sh) {
     using L = Layout<D, Q>;
     constexpr int ROWS = 16 * MT, WT = L::WT, NT = WT / 8, KS = D / 16, DT = D / 8;
     constexpr bool Q_IN_REGS = MT * D <= 128;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int gq = lane >> 2, tq = lane & 3;
-    const int n_tok = t1 - t0, n_tiles = (n_tok + L::TILE - 1) / L::TILE;
-
     uint8_t* sq = smem;
     uint32_t* place = reinterpret_cast<uint32_t*>(sq + ROWS * D * 2);
     uint32_t* tok_scale = place + src.chunk;  // Int8: bf16 (k, v) scales of each token
@@ -110,6 +111,8 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
     volatile int* abort_flag = &sh.abort_flag;
 
     // ---- where each token of the chunk lies, and the query rows ----
+    // The loads of either half of the CTA are under way together: those of the table do not wait for the length (an entry
+    // below max_len exists, what it holds is used only below the length), the copies not for scales and query rows.
     if (tid == 0) {
         for (int s = 0; s < L::STAGES; ++s) {
             izb::mbar_init(izb::smem_u32(&sh.full[s]), 128);
@@ -118,37 +121,55 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
         sh.abort_flag = 0;
         izb::mbar_fence_init();
     }
-    for (int i = tid; i < n_tiles * L::TILE; i += SP_THREADS) {
-        uint32_t at = 0, sc = 0;  // tokens past the chunk: a place that can be addressed, a zero scale
-        if (i < n_tok) {
-            const int t = t0 + i, pg = t / src.page_size;
-            const int page = src.table[static_cast<long long>(src_row) * src.max_pages + pg];
-            at = static_cast<uint32_t>(page) * static_cast<uint32_t>(src.page_size) + static_cast<uint32_t>(t - pg * src.page_size);
-            if (Q == IZB_KV_INT8) sc = izb::pack_bf16x2(src.k_scales[page], src.v_scales[page]);
+    constexpr int U = SP_MAX_CHUNK / 128, QV = ROWS * (D / 8) / 128;
+    const int t128 = tid & 127;
+    const int first_page = (t0 + t128) / src.page_size, first_rest = t0 + t128 - first_page * src.page_size;
+    int pages[U];
+    if (warp >= 4 || Q == IZB_KV_INT8) {
+        const int* table = src.table + static_cast<long long>(src_row) * src.max_pages;
+        int pg = first_page, rest = first_rest;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = u * 128 + t128;
+            pages[u] = 0;
+            if (i < src.chunk && t0 + i < src.max_len) pages[u] = table[pg];
+            pg += src.step_pages;
+            rest += src.step_rest;
+            if (rest >= src.page_size) { rest -= src.page_size; ++pg; }
         }
-        place[i] = at;
-        if (Q == IZB_KV_INT8) tok_scale[i] = sc;
     }
-    for (int i = tid; i < ROWS * (D / 8); i += SP_THREADS) {
-        const int r = i / (D / 8), c = i % (D / 8), row = row0 + r;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (r < n_rows) {
-            const int s = row / p.g, h = row - s * p.g;
-            v = *reinterpret_cast<const uint4*>(p.q + (seq0 + s) * p.ld_q + static_cast<long long>(kh * p.g + h) * D + c * 8);
-            v.x ^= p.q_sign; v.y ^= p.q_sign; v.z ^= p.q_sign; v.w ^= p.q_sign;
+    uint4 qv[QV];
+    if (warp < 4) {
+#pragma unroll
+        for (int u = 0; u < QV; ++u) {
+            const int i = u * 128 + tid, r = i / (D / 8), c = i % (D / 8), row = row0 + r;
+            qv[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (r < n_rows) {
+                const int s = row / p.g, h = row - s * p.g;
+                qv[u] = *reinterpret_cast<const uint4*>(p.q + (seq0 + s) * p.ld_q + static_cast<long long>(kh * p.g + h) * D + c * 8);
+            }
         }
-        // Q4_0 codes leave their words as the channel pairs (0, 4), (1, 5), (2, 6), (3, 7) of eight
-        if (Q == IZB_KV_Q4_0)
-            v = make_uint4(izb::prmt(v.x, v.z, 0x5410), izb::prmt(v.x, v.z, 0x7632), izb::prmt(v.y, v.w, 0x5410), izb::prmt(v.y, v.w, 0x7632));
-        *reinterpret_cast<uint4*>(sq + r * D * 2 + ((c ^ (r & 7)) << 4)) = v;
     }
+    const int n_tok = min(length_of(src, src_row) - t0, src.chunk);
+    if (n_tok <= 0) return;
+    const int n_tiles = (n_tok + L::TILE - 1) / L::TILE;
     __syncthreads();
 
     bool ok = true;
     if (warp >= 4) {
         // ---------------- copies ----------------
+        int rest = first_rest;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = u * 128 + t128;  // tokens past the chunk: a place that can be addressed
+            if (i < n_tiles * L::TILE)
+                place[i] = i < n_tok ? static_cast<uint32_t>(pages[u]) * static_cast<uint32_t>(src.page_size) + static_cast<uint32_t>(rest) : 0u;
+            rest += src.step_rest;
+            if (rest >= src.page_size) rest -= src.page_size;
+        }
+        izb::named_bar_sync(2, 128);
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(COPY_REGS));
-        const int t = tid - 128;
+        const int t = t128;
         constexpr int RSTEP = 128 / L::CHUNKS;  // rows the 128 threads take at a time, a 16-byte chunk each
         const int my_r = t / L::CHUNKS, my_c = t % L::CHUNKS;
         const uint32_t stride = static_cast<uint32_t>(p.kv_heads) * L::ROW;
@@ -192,6 +213,34 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
         return;
     }
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<D, MT_LAUNCH>::COMPUTE));
+    if (Q == IZB_KV_INT8) {
+        float ks[U], vs[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            ks[u] = vs[u] = 0.f;
+            if (u * 128 + tid < n_tok) {
+                ks[u] = src.k_scales[pages[u]];
+                vs[u] = src.v_scales[pages[u]];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)  // zero past the chunk
+            if (u * 128 + tid < n_tiles * L::TILE) tok_scale[u * 128 + tid] = izb::pack_bf16x2(ks[u], vs[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < QV; ++u) {
+        const int i = u * 128 + tid, r = i / (D / 8), c = i % (D / 8);
+        uint4 v = make_uint4(qv[u].x ^ p.q_sign, qv[u].y ^ p.q_sign, qv[u].z ^ p.q_sign, qv[u].w ^ p.q_sign);
+        // Q4_0 codes leave their words as the channel pairs (0, 4), (1, 5), (2, 6), (3, 7) of eight
+        if (Q == IZB_KV_Q4_0)
+            v = make_uint4(izb::prmt(v.x, v.z, 0x5410), izb::prmt(v.x, v.z, 0x7632), izb::prmt(v.y, v.w, 0x5410), izb::prmt(v.y, v.w, 0x7632));
+        *reinterpret_cast<uint4*>(sq + r * D * 2 + ((c ^ (r & 7)) << 4)) = v;
+    }
+    if (tid < n_rows) {
+        const int row = row0 + tid, s = row / p.g, h = row - s * p.g;
+        sh.slot[tid] = (static_cast<long long>(seq0 + s) * p.heads + kh * p.g + h) * chunks_total + chunk_slot;
+    }
+    izb::named_bar_sync(1, 128);
     float o[MT][DT][4], m[MT][2], l[MT][2];
     {
         const CodeBits<Q> bits;
@@ -452,7 +501,10 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
     izb::named_bar_sync(1, 128);  // every tile of the ring has been read; from here on the four computing warps alone
 
     // ---- join the warps, leave the chunk's result ----
-    constexpr int LD = D + 4;
+    // Codes leave a lane with runs of D / 8 channels; run n is turned by n 16-byte columns, so that the eight lanes of a
+    // store phase (two rows, four runs) meet different banks.
+    constexpr int LD = L::EX_LD;
+    auto turned = [](int col) { return D == 128 ? col ^ (col >> 2) : col ^ ((col >> 3) << 1); };
     float* ex = reinterpret_cast<float*>(ring);  // [warp][16 MT][LD]
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -467,14 +519,10 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
                     for (int j = 0; j < DT; j += 4)
-                        *reinterpret_cast<float4*>(row + (tq * 2 + e) * DT + j) =
+                        *reinterpret_cast<float4*>(row + turned(((tq * 2 + e) * DT + j) / 4) * 4) =
                             make_float4(o[mt][j][h * 2 + e], o[mt][j + 1][h * 2 + e], o[mt][j + 2][h * 2 + e], o[mt][j + 3][h * 2 + e]);
             }
         }
-    auto slot_of = [&](int r) {
-        const int row = row0 + r, s = row / p.g, h = row - s * p.g;
-        return (static_cast<long long>(seq0 + s) * p.heads + kh * p.g + h) * chunks_total + chunk_slot;
-    };
     if (tid < n_rows) {
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
@@ -486,19 +534,20 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
             sh.factor[w][tid] = f;
             sum += f * x.y;
         }
-        p.ml[slot_of(tid)] = make_float2(top * p.scale_log2, sum);
+        p.ml[sh.slot[tid]] = make_float2(top * p.scale_log2, sum);
     }
     izb::named_bar_sync(1, 128);
+#pragma unroll 4
     for (int i = tid; i < n_rows * (D / 4); i += 128) {
-        const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+        const int r = i / (D / 4), col = i % (D / 4), at = Q == IZB_KV_NONE ? col : turned(col);
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const float f = sh.factor[w][r];
-            const float4 x = *reinterpret_cast<const float4*>(ex + (w * ROWS + r) * LD + d);
+            const float4 x = *reinterpret_cast<const float4*>(ex + (w * ROWS + r) * LD + at * 4);
             a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
         }
-        *reinterpret_cast<float4*>(p.acc + slot_of(r) * D + d) = a;
+        *reinterpret_cast<float4*>(p.acc + sh.slot[r] * D + col * 4) = a;
     }
 }
 
@@ -517,27 +566,23 @@ __global__ void __launch_bounds__(SP_THREADS, Regs<D, MT>::CTAS) shared_prefix_k
         const int kh = item % p.kv_heads;
         item /= p.kv_heads;
         const int chunk = item % p.prefix.n_chunks, group = item / p.prefix.n_chunks;
-        const int len = length_of(p.prefix, group), t0 = chunk * p.prefix.chunk, t1 = min(len, t0 + p.prefix.chunk);
-        if (t0 >= t1) return;
-        const int row0 = rb * 16 * MT, n = min(16 * MT, p.seqs * p.g - row0);
+        const int t0 = chunk * p.prefix.chunk, row0 = rb * 16 * MT, n = min(16 * MT, p.seqs * p.g - row0);
         if (p.prefix.quant == IZB_KV_NONE)
-            attend<D, MT, IZB_KV_NONE, MT>(p, p.prefix, group, kh, group * p.seqs, row0, n, t0, t1, chunk, chunks, smem, sh);
+            attend<D, MT, IZB_KV_NONE, MT>(p, p.prefix, group, kh, group * p.seqs, row0, n, t0, chunk, chunks, smem, sh);
         else if (p.prefix.quant == IZB_KV_INT8)
-            attend<D, MT, IZB_KV_INT8, MT>(p, p.prefix, group, kh, group * p.seqs, row0, n, t0, t1, chunk, chunks, smem, sh);
+            attend<D, MT, IZB_KV_INT8, MT>(p, p.prefix, group, kh, group * p.seqs, row0, n, t0, chunk, chunks, smem, sh);
         else
-            attend<D, MT, IZB_KV_Q4_0, MT>(p, p.prefix, group, kh, group * p.seqs, row0, n, t0, t1, chunk, chunks, smem, sh);
+            attend<D, MT, IZB_KV_Q4_0, MT>(p, p.prefix, group, kh, group * p.seqs, row0, n, t0, chunk, chunks, smem, sh);
         return;
     }
     item -= p.prefix_items;
     const int kh = item % p.kv_heads;
     item /= p.kv_heads;
     const int chunk = item % p.own.n_chunks, seq = item / p.own.n_chunks;
-    const int len = length_of(p.own, seq), t0 = chunk * p.own.chunk, t1 = min(len, t0 + p.own.chunk);
-    if (t0 >= t1) return;
-    const int slot = p.prefix.n_chunks + chunk;
-    if (p.own.quant == IZB_KV_NONE) attend<D, 1, IZB_KV_NONE, MT>(p, p.own, seq, kh, seq, 0, p.g, t0, t1, slot, chunks, smem, sh);
-    else if (p.own.quant == IZB_KV_INT8) attend<D, 1, IZB_KV_INT8, MT>(p, p.own, seq, kh, seq, 0, p.g, t0, t1, slot, chunks, smem, sh);
-    else attend<D, 1, IZB_KV_Q4_0, MT>(p, p.own, seq, kh, seq, 0, p.g, t0, t1, slot, chunks, smem, sh);
+    const int t0 = chunk * p.own.chunk, slot = p.prefix.n_chunks + chunk;
+    if (p.own.quant == IZB_KV_NONE) attend<D, 1, IZB_KV_NONE, MT>(p, p.own, seq, kh, seq, 0, p.g, t0, slot, chunks, smem, sh);
+    else if (p.own.quant == IZB_KV_INT8) attend<D, 1, IZB_KV_INT8, MT>(p, p.own, seq, kh, seq, 0, p.g, t0, slot, chunks, smem, sh);
+    else attend<D, 1, IZB_KV_Q4_0, MT>(p, p.own, seq, kh, seq, 0, p.g, t0, slot, chunks, smem, sh);
 }
 
 // One CTA per (sequence, head): four warps take every fourth chunk, a lane D / 32 channels.
@@ -674,6 +719,8 @@ int source_from(const izb_kv_pages* a, const int32_t* lens, int64_t max_len, Sou
     s->max_pages = a->max_pages_per_seq;
     s->quant = a->quantization;
     s->page_size = a->page_size;
+    s->step_pages = 128 / a->page_size;
+    s->step_rest = 128 % a->page_size;
     s->max_len = static_cast<int>(max_len);
     return IZB_OK;
 }

@@ -20,6 +20,7 @@ struct Source {
     int max_len;     // lengths on the device are cut to this
     int chunk;       // tokens per item
     int n_chunks;    // partial results a row can have from this cache
+    int step_pages, step_rest;  // 128 tokens in pages and what is left of them
 };
 
 struct Params {
