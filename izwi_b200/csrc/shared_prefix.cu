@@ -9,7 +9,7 @@
 //
 // Work: an item is (group, KV head, block of query rows, chunk of prefix tokens) or (sequence, KV head, chunk of its
 // own tokens); all items go out in one launch, one CTA each, or, with many rows or a long prefix, those of the prefix in
-// a launch of their own on tensor memory (shared_prefix_tc.cu).  A CTA walks its chunk in tiles with a running maximum
+// a launch of their own on tensor memory (shared_prefix_tc.cu), behind which short own tokens join the last launch.  A CTA walks its chunk in tiles with a running maximum
 // and sum per row and leaves (max, sum, weighted values) for a last launch that joins the chunks
 // of every (sequence, head).  fp32 for scores, maxima, sums and accumulators; p is rounded to bf16 for the product
 // with v (half a step: 2^-9 relative, independent per token, which is what the bf16 output itself carries).
@@ -81,13 +81,51 @@ struct Regs {
     static constexpr int COMPUTE = 2 * LAUNCH - COPY_REGS;
 };
 
+struct Result {
+    __nv_bfloat16* out;
+    long long ld;
+};
+
 struct ItemShared {
     unsigned long long full[4], empty[4];
     long long slot[32];   // per row: its place among the partial results
     float2 wml[4][32];    // per warp and row: maximum and sum
     float factor[4][32];  // per warp and row: weight in the joined result
+    float2 own[SP_MAX_G];  // of an item that finishes its rows: maximum (log2 scale) and sum
     int abort_flag;
 };
+
+// Chunks of the prefix a row of `group` has partial results of.
+__device__ __forceinline__ int prefix_chunks_of(const Params& p, int group) {
+    return p.prefix.n_chunks ? (length_of(p.prefix, group) + p.prefix.chunk - 1) / p.prefix.chunk : 0;
+}
+
+// `a`: weighted values of channels col * 4.. under maximum m (log2 scale) and sum l, joined with the row's partial results
+// of the prefix from `slot` on; leaves the row's result.
+template <int D>
+__device__ __forceinline__ void finish(const Params& p, const Result& to, float4 a, float m, float l, long long slot, int np, int seq, int head,
+                                       int col) {
+#pragma unroll 6
+    for (int c = 0; c < np; ++c) {
+        const float2 x = p.ml[slot + c];
+        const float4 v = *reinterpret_cast<const float4*>(p.acc + (slot + c) * D + col * 4);
+        const float n = fmaxf(m, x.x), u = n == -INFINITY ? 0.f : n;
+        const float f = ex2(m - u), g = ex2(x.x - u);
+        l = l * f + x.y * g;
+        m = n;
+        a = make_float4(a.x * f + v.x * g, a.y * f + v.y * g, a.z * f + v.z * g, a.w * f + v.w * g);
+    }
+    // a row without any token gives zeros; NaN in a sum is not hidden
+    const float4 y = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(a.x / l, a.y / l, a.z / l, a.w / l);
+    __nv_bfloat16* out = to.out + seq * to.ld + static_cast<long long>(head) * D + col * 4;
+    const uint32_t lo = izb::pack_bf16x2(y.x, y.y), hi = izb::pack_bf16x2(y.z, y.w);
+    if ((reinterpret_cast<uintptr_t>(out) & 7) == 0) {
+        *reinterpret_cast<uint2*>(out) = make_uint2(lo, hi);
+    } else {
+        const __nv_bfloat162 b[2] = {*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&hi)};
+        out[0] = b[0].x; out[1] = b[0].y; out[2] = b[1].x; out[3] = b[1].y;
+    }
+}
 
 // One item: n_rows (at most 16 MT) query rows from row0 that meet KV head kh of `src` row `src_row`, a chunk of tokens from t0.
 // Warps 0..3 compute, each on its share of every tile with a maximum, sum and accumulator of its own; warps 4..7
@@ -95,9 +133,10 @@ struct ItemShared {
 // registers the copying warps do not need go to the computing ones (setmaxnreg; their shares add up to the launch's).
 //   Scores and outputs are mma.sync products of 16 rows: with at most 32 rows a 128-row tensor-memory tile would be idle
 // for three quarters of its rows, while here a tile's fragments are read (or made from codes) exactly once.
-template <int D, int MT, int Q, int MT_LAUNCH>
+//   FINISH: the item holds all own tokens of its rows and the prefix is done; it leaves the rows' results.
+template <int D, int MT, int Q, int MT_LAUNCH, bool FINISH = false>
 __device__ __forceinline__ void attend(const Params& p, const Source& src, int src_row, int kh, int seq0, int row0, int n_rows, int t0,
-                                       int chunk_slot, int chunks_total, uint8_t* smem, ItemShared& sh) {
+                                       int chunk_slot, int chunks_total, uint8_t* smem, ItemShared& sh, const Result& to = Result{}) {
     using L = Layout<D, Q>;
     constexpr int ROWS = 16 * MT, WT = L::WT, NT = WT / 8, KS = D / 16, DT = D / 8;
     constexpr bool Q_IN_REGS = MT * D <= 128;
@@ -151,7 +190,16 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
         }
     }
     const int n_tok = min(length_of(src, src_row) - t0, src.chunk);
-    if (n_tok <= 0) return;
+    const int np = FINISH ? prefix_chunks_of(p, seq0 / p.seqs) : 0;
+    if (n_tok <= 0) {
+        if (FINISH)
+            for (int i = tid; i < n_rows * (D / 4); i += SP_THREADS) {
+                const int r = i / (D / 4), head = kh * p.g + r;
+                finish<D>(p, to, make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f, (static_cast<long long>(seq0) * p.heads + head) * chunks_total, np, seq0, head,
+                          i % (D / 4));
+            }
+        return;
+    }
     const int n_tiles = (n_tok + L::TILE - 1) / L::TILE;
     __syncthreads();
 
@@ -534,7 +582,8 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
             sh.factor[w][tid] = f;
             sum += f * x.y;
         }
-        p.ml[sh.slot[tid]] = make_float2(top * p.scale_log2, sum);
+        if (FINISH) sh.own[tid] = make_float2(top * p.scale_log2, sum);
+        else p.ml[sh.slot[tid]] = make_float2(top * p.scale_log2, sum);
     }
     izb::named_bar_sync(1, 128);
 #pragma unroll 4
@@ -547,7 +596,8 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
             const float4 x = *reinterpret_cast<const float4*>(ex + (w * ROWS + r) * LD + at * 4);
             a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
         }
-        *reinterpret_cast<float4*>(p.acc + sh.slot[r] * D + col * 4) = a;
+        if constexpr (FINISH) finish<D>(p, to, a, sh.own[r].x, sh.own[r].y, sh.slot[r] - chunk_slot, np, seq0, kh * p.g + r, col);
+        else *reinterpret_cast<float4*>(p.acc + sh.slot[r] * D + col * 4) = a;
     }
 }
 
@@ -585,6 +635,22 @@ __global__ void __launch_bounds__(SP_THREADS, Regs<D, MT>::CTAS) shared_prefix_k
     else attend<D, 1, IZB_KV_Q4_0, MT>(p, p.own, seq, kh, seq, 0, p.g, t0, slot, chunks, smem, sh);
 }
 
+// Behind the tensor-memory kernel: an item per (sequence, KV head) takes the sequence's own tokens, joins the chunks of the
+// prefix and leaves the result, where there are few enough own tokens for one item.  (In a launch before it they cost that
+// launch, and this one the reading of their partial results: 64 sequences of up to 256 own tokens 68.7 us against 64.2.)
+template <int D>
+__global__ void __launch_bounds__(SP_THREADS, Regs<D, 1>::CTAS) shared_prefix_finish_kernel(const __grid_constant__ Params p, const __grid_constant__ Result to) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ ItemShared sh;
+    izb::pdl_launch_dependents();
+    izb::pdl_wait();
+    const int chunks = p.prefix.n_chunks + p.own.n_chunks;
+    const int kh = blockIdx.x % p.kv_heads, seq = blockIdx.x / p.kv_heads;
+    if (p.own.quant == IZB_KV_NONE) attend<D, 1, IZB_KV_NONE, 1, true>(p, p.own, seq, kh, seq, 0, p.g, 0, p.prefix.n_chunks, chunks, smem, sh, to);
+    else if (p.own.quant == IZB_KV_INT8) attend<D, 1, IZB_KV_INT8, 1, true>(p, p.own, seq, kh, seq, 0, p.g, 0, p.prefix.n_chunks, chunks, smem, sh, to);
+    else attend<D, 1, IZB_KV_Q4_0, 1, true>(p, p.own, seq, kh, seq, 0, p.g, 0, p.prefix.n_chunks, chunks, smem, sh, to);
+}
+
 // One CTA per (sequence, head): four warps take every fourth chunk, a lane D / 32 channels.
 template <int D>
 __global__ void __launch_bounds__(128)
@@ -596,7 +662,7 @@ __global__ void __launch_bounds__(128)
     const int row = blockIdx.x, seq = row / p.heads, head = row - seq * p.heads;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int chunks = p.prefix.n_chunks + p.own.n_chunks;
-    const int np = p.prefix.n_chunks ? (length_of(p.prefix, seq / p.seqs) + p.prefix.chunk - 1) / p.prefix.chunk : 0;
+    const int np = prefix_chunks_of(p, seq / p.seqs);
     const int no = p.own.n_chunks ? (length_of(p.own, seq) + p.own.chunk - 1) / p.own.chunk : 0;
     const long long base = static_cast<long long>(row) * chunks;
     float m = -INFINITY, l = 0.f, a[E];
@@ -641,6 +707,7 @@ __global__ void __launch_bounds__(128)
 // ---- host side ---------------------------------------------------------------------------------------------------
 struct Plan {
     bool tc;         // the prefix goes to the tensor-memory kernel
+    bool own_finishes;  // the own tokens are taken behind it, by the launch that joins
     int rows;        // query rows of a prefix item
     int row_blocks;
     int prefix_chunk, prefix_chunks, own_chunk, own_chunks;
@@ -665,20 +732,23 @@ int choose_chunk(int64_t base, int64_t tokens, int64_t slots, int tile, int extr
     return static_cast<int>(best * tile);
 }
 
-Plan make_plan(const izb_ctx* ctx, int64_t groups, int64_t seqs, int kv_heads, int g, int head_dim, bool bf16, int64_t max_prefix, int64_t max_own) {
+Plan make_plan(const izb_ctx* ctx, int64_t groups, int64_t seqs, int kv_heads, int g, int head_dim, int quant, int64_t max_prefix, int64_t max_own) {
     Plan pl = {};
     const int64_t rows = seqs * g, sms = ctx && ctx->sm_count > 0 ? ctx->sm_count : 148;
     // Which kernel takes the prefix.  Above 32 rows a second block of 32 would read the tiles again, and the tensor-memory
     // kernel holds 128 or 256.  Up to 32 its rows are mostly idle, but a 128-token bf16 tile of D = 128 takes it 1,900
     // cycles against 3,300 to 4,900 here; against that stand some 5 us for an item's first loads, tensor memory and result,
     // so items have to be long (bf16, 32,768 tokens, 2 x 8 heads: 16 rows 53.8 us against 64.7, 32 rows 54.3 against 73.8;
-    // 12 tiles an item, 5 rows: 118 against 94).  Converting codes takes it 4,200 cycles a tile, which pays from 17 rows
-    // (Int8, 32,768 tokens, 2 x 8 heads, 32 rows: 73 against 85; at 8 tiles an item level, and then one launch for prefix
-    // and own pages is better than two); D = 64: 35 us against 18.5 at 12 tiles an item.
+    // 12 tiles an item, 5 rows: 118 against 94).  Codes are converted there by warps of their own, which pays from 17 rows:
+    // Q4_0, whose conversion takes most, at any length (4 x 8 beams, 32 rows, 131 own tokens: 1,000 tokens 21.6 us against
+    // 24.5, 4,099 31.5 against 32.9, 8,192 43.1 against 59.1), Int8 for long items (9 tiles an item 32.4 against 30.0, 16 tiles
+    // 47.3 against 47.8, 33 tiles 69.7 against 77.5); with 16 rows 16,384 tokens of Int8 take 52.9 against 48.3.  D = 64: 54 us
+    // against 31 (bf16), 64 against 48 (Int8, 30 rows) at 12 tiles an item.
     const int tc_rows = rows <= TC_ROWS ? TC_ROWS : 2 * TC_ROWS;
     const int64_t tc_items = groups * kv_heads * ((rows + tc_rows - 1) / tc_rows);
     const int tc_chunk = max_prefix > 0 ? choose_chunk(tc_items, max_prefix, sms, 128, 4, 1 << 20) : 0;
-    pl.tc = rows > 32 || (head_dim == 128 && (rows > 16 ? tc_chunk >= 12 * 128 : bf16 && tc_chunk >= 16 * 128));
+    const int least = rows > 16 ? (quant == IZB_KV_Q4_0 ? 2 : 12) : quant == IZB_KV_NONE ? 16 : 1 << 20;
+    pl.tc = rows > 32 || (head_dim == 128 && tc_chunk >= least * 128);
     pl.rows = pl.tc ? tc_rows : rows <= 16 ? 16 : 32;
     pl.row_blocks = static_cast<int>((rows + pl.rows - 1) / pl.rows);
     const int64_t slots = (head_dim == 64 && (rows <= 16 || pl.tc) ? 3 : 2) * sms;  // of the other kernel
@@ -691,6 +761,7 @@ Plan make_plan(const izb_ctx* ctx, int64_t groups, int64_t seqs, int kv_heads, i
         pl.own_chunk = choose_chunk(groups * seqs * kv_heads, max_own, slots, SP_TILE, 1, SP_MAX_CHUNK / SP_TILE);
         pl.own_chunks = static_cast<int>((max_own + pl.own_chunk - 1) / pl.own_chunk);
     }
+    pl.own_finishes = pl.tc && pl.own_chunks == 1;
     return pl;
 }
 
@@ -732,13 +803,9 @@ size_t smem_for(const Source& s) {
            : s.quant == IZB_KV_INT8 ? item_smem<D, MT, IZB_KV_INT8>(s.chunk) : item_smem<D, MT, IZB_KV_Q4_0>(s.chunk);
 }
 
-template <int D, int MT>
-int launch_items(izb_ctx* ctx, cudaStream_t s, const Params& p, int64_t items) {
-    size_t smem = p.prefix_items > 0 ? smem_for<D, MT>(p.prefix) : 0;
-    const size_t own = smem_for<D, 1>(p.own);
-    if (own > smem) smem = own;
-    auto kern = shared_prefix_kernel<D, MT>;
-    static std::atomic<bool> ready[IZB_MAX_DEVICES];
+template <int D, int MT, typename... Args>
+int launch_items(izb_ctx* ctx, cudaStream_t s, void (*kern)(Params, Args...), std::atomic<bool>* ready, size_t smem, int64_t items, const Params& p,
+                 const Args&... args) {
     if (!ready[ctx->device].load(std::memory_order_relaxed)) {
         cudaFuncAttributes attr;
         IZB_CUDA_TRY(cudaFuncGetAttributes(&attr, kern));
@@ -746,21 +813,32 @@ int launch_items(izb_ctx* ctx, cudaStream_t s, const Params& p, int64_t items) {
         IZB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ctx->max_smem_optin - static_cast<int>(attr.sharedSizeBytes)));
         ready[ctx->device].store(true, std::memory_order_relaxed);
     }
-    IZB_CUDA_TRY(izb::launch_chained(ctx, kern, dim3(static_cast<unsigned>(items)), dim3(SP_THREADS), smem, s, p));
+    IZB_CUDA_TRY(izb::launch_chained(ctx, kern, dim3(static_cast<unsigned>(items)), dim3(SP_THREADS), smem, s, p, args...));
     ctx->launches.fetch_add(1, std::memory_order_relaxed);
     return IZB_OK;
+}
+
+template <int D, int MT>
+int launch_all_items(izb_ctx* ctx, cudaStream_t s, const Params& p, int64_t items) {
+    static std::atomic<bool> ready[IZB_MAX_DEVICES];
+    const size_t prefix = p.prefix_items > 0 ? smem_for<D, MT>(p.prefix) : 0, own = smem_for<D, 1>(p.own);
+    return launch_items<D, MT>(ctx, s, shared_prefix_kernel<D, MT>, ready, prefix > own ? prefix : own, items, p);
 }
 
 template <int D>
 int launch_dim(izb_ctx* ctx, cudaStream_t s, const Params& p, const Plan& pl, int64_t items, int64_t batch, __nv_bfloat16* out,
                long long ld_out) {
     if (items > 0) {
-        const int rc = pl.tc || pl.rows == 16 ? launch_items<D, 1>(ctx, s, p, items) : launch_items<D, 2>(ctx, s, p, items);
+        const int rc = pl.tc || pl.rows == 16 ? launch_all_items<D, 1>(ctx, s, p, items) : launch_all_items<D, 2>(ctx, s, p, items);
         if (rc != IZB_OK) return rc;
     }
     if (pl.tc && p.prefix.n_chunks > 0) {
         const int rc = launch_prefix_tc(ctx, s, p, D, batch / p.seqs);
         if (rc != IZB_OK) return rc;
+    }
+    if (pl.own_finishes) {
+        static std::atomic<bool> ready[IZB_MAX_DEVICES];
+        return launch_items<D, 1>(ctx, s, shared_prefix_finish_kernel<D>, ready, smem_for<D, 1>(p.own), batch * p.kv_heads, p, Result{out, ld_out});
     }
     IZB_CUDA_TRY(izb::launch_chained(ctx, shared_prefix_join_kernel<D>, dim3(static_cast<unsigned>(batch * p.heads)), dim3(128), 0, s, p, out,
                                      ld_out));
@@ -778,10 +856,10 @@ size_t izb_shared_prefix_decode_gqa_attention_workspace_bytes(const izb_ctx* ctx
     if (groups <= 0 || seqs_per_group <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || head_dim <= 0 ||
         max_prefix_len < 0 || max_seq_len < 0 || groups > INT32_MAX / seqs_per_group || max_prefix_len > INT32_MAX || max_seq_len > INT32_MAX)
         return 0;
-    // the query does not know how the pages are stored: enough for either plan
+    // the query does not know how the pages are stored: enough for every plan
     size_t most = 0;
-    for (int bf16 = 0; bf16 < 2; ++bf16) {
-        const Plan pl = make_plan(ctx, groups, seqs_per_group, kv_heads, heads / kv_heads, head_dim, bf16 != 0, max_prefix_len, max_seq_len);
+    for (int quant = IZB_KV_NONE; quant <= IZB_KV_Q4_0; ++quant) {
+        const Plan pl = make_plan(ctx, groups, seqs_per_group, kv_heads, heads / kv_heads, head_dim, quant, max_prefix_len, max_seq_len);
         const size_t need = plan_bytes(pl, groups * seqs_per_group, heads, head_dim);
         most = need > most ? need : most;
     }
@@ -811,7 +889,7 @@ int32_t izb_shared_prefix_decode_gqa_attention(izb_ctx* ctx, izb_stream stream, 
     if (ld_q < static_cast<int64_t>(heads) * d || ld_out < static_cast<int64_t>(heads) * d) return IZB_ERR_BAD_ARG;
     if (groups > INT32_MAX / seqs_per_group || groups * seqs_per_group > INT32_MAX / heads) return IZB_ERR_UNSUPPORTED;
     const int64_t batch = groups * seqs_per_group;
-    const Plan pl = make_plan(ctx, groups, seqs_per_group, kv_heads, heads / kv_heads, d, p.prefix.quant == IZB_KV_NONE, max_prefix_len, max_seq_len);
+    const Plan pl = make_plan(ctx, groups, seqs_per_group, kv_heads, heads / kv_heads, d, p.prefix.quant, max_prefix_len, max_seq_len);
     const size_t need = plan_bytes(pl, batch, heads, d);
     if (need && (!workspace || workspace_bytes < need || !izb_aligned(workspace, 16))) return IZB_ERR_BAD_ARG;
     p.prefix.chunk = pl.prefix_chunk;
@@ -831,8 +909,8 @@ int32_t izb_shared_prefix_decode_gqa_attention(izb_ctx* ctx, izb_stream stream, 
     p.q_sign = scale < 0.f ? 0x80008000u : 0u;
     p.scale_log2 = fmaxf(fabsf(scale) * LOG2E, 1e-30f);  // not 0: a masked product is -inf and must stay it
     p.margin = 8.f / p.scale_log2;
-    const int64_t prefix_items = pl.tc ? 0 : groups * pl.prefix_chunks * kv_heads * pl.row_blocks, items = prefix_items + batch * kv_heads * pl.own_chunks;
-    if (items > INT32_MAX || groups * pl.prefix_chunks > INT32_MAX / kv_heads / pl.row_blocks) return IZB_ERR_UNSUPPORTED;
+    const int64_t prefix_items = pl.tc ? 0 : groups * pl.prefix_chunks * kv_heads * pl.row_blocks, items = prefix_items + (pl.own_finishes ? 0 : batch * kv_heads * pl.own_chunks);
+    if (items > INT32_MAX || batch * kv_heads > INT32_MAX || groups * pl.prefix_chunks > INT32_MAX / kv_heads / pl.row_blocks) return IZB_ERR_UNSUPPORTED;
     p.prefix_items = static_cast<int>(prefix_items);
     izb::DeviceGuard guard(ctx->device);
     if (!guard.ok) return IZB_ERR_LAUNCH;

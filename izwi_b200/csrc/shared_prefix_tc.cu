@@ -10,10 +10,8 @@
 // every tile serves both, so that the prefix is read once for 256 rows.
 //   warps 0..3, 4..7   weights of set 0, 1: a thread owns a row
 //   bf16 pages:  warp 8 fetches tiles (TMA, four token rows of a paged pool at a time), warp 9 issues the products
-//   codes:       warps 8..15 convert tiles through registers, once for all rows; warp 16 issues the products
+//   codes:       four or eight warps convert K and as many V through registers, once for all rows; the next issues the products
 // Rows of a tile are 128-byte swizzle rows, 64 channels each: K is the K-major operand, V the same bytes read MN-major.
-#include <climits>
-
 #include "shared_prefix.cuh"
 #include "tcgen05.cuh"
 #include "tma.cuh"
@@ -23,23 +21,26 @@ namespace shared_prefix {
 namespace {
 
 constexpr int TC_TILE = 128;                    // tokens
-constexpr int TC_COPY = 256;                    // converting threads
-constexpr int TC_CALLED = 3;                    // tiles ahead of the conversion that are called into L2
-// Threads and, for codes, registers: 640 threads of 96 at launch become 256 x 128 + 256 x 88 + 128 x 48 = 640 x 96.  bf16:
-// 384 threads of 168, enough for a row's 128 scores at once.
-constexpr int TC_WEIGHT_REGS = 128, TC_COPY_REGS = 88, TC_ISSUE_REGS = 48, TC_LAUNCH_REGS = 96;
-constexpr int tc_threads(int quant) { return quant == IZB_KV_NONE ? 384 : 256 + TC_COPY + 128; }
+// Threads and registers.  bf16 pages: 384 threads of 168, enough for a row's 128 scores at once.  Codes: CONV threads convert
+// K and as many V, and the launch's registers are shared out: 640 x 96 = 256 x 128 + 256 x 88 + 128 x 48 (CONV = 128),
+// 896 x 72 = 256 x 112 + 512 x 64 + 128 x 24 (CONV = 256).
+template <int Q, int CONV>
+struct Roles {
+    static constexpr bool CODES = Q != IZB_KV_NONE;
+    static constexpr int THREADS = CODES ? 256 + 2 * CONV + 128 : 384;
+    static constexpr int ISSUE_WARP = CODES ? 8 + 2 * CONV / 32 : 9;
+    static constexpr int LAUNCH = !CODES ? 168 : CONV == 128 ? 96 : 72, WEIGHTS = CONV == 128 ? 128 : 112, COPY = CONV == 128 ? 88 : 64,
+                         ISSUE = CONV == 128 ? 48 : 24;
+    static_assert(!CODES || 256 * WEIGHTS + 2 * CONV * COPY + 128 * ISSUE <= THREADS * LAUNCH, "registers that nobody has");
+};
 constexpr int TC_HALF = TC_TILE * 128;          // bytes of 64 channels of a tile
 
 struct TcShared {
     unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2];
-    unsigned long long s_full[2], p_full[2][2], pv_done[2];  // p_full: per set and half of a tile's tokens
-    uint32_t place[4][TC_TILE];  // per tile, four in turn: pool token of each tile token
-    uint32_t page[4][TC_TILE];   // Int8: its page
+    unsigned long long s_full[2], p_full[2][2], pv_done[2][2];  // per set and half of a tile's tokens
     unsigned long long q_full;
     float2 ml[2][128];           // narrow blocks: maximum and sum of a row in either set
     uint32_t tmem;
-    int copy_failed;  // the unit at which a wait gave up
     int failed;       // some wait gave up
 };
 
@@ -201,150 +202,141 @@ __device__ __forceinline__ void fetch_role(const Params& p, const Maps& maps, in
     }
 }
 
-// Codes.  Units of the stream: K of tile 0, V of tile 0, K of tile 1, ...  Slot (tile & 1) of either ring.
-template <int D, int Q>
-__device__ __forceinline__ void convert_role(const Params& p, int src_row, int kh, int t0, int n_tok, uint32_t k_ring, uint32_t v_ring, TcShared& sh) {
-    constexpr int ROW = Q == IZB_KV_INT8 ? D : D / 2;
-    constexpr int CHUNKS = ROW / 16, RSTEP = TC_COPY / CHUNKS, N = TC_TILE / RSTEP;  // chunks of a unit per thread
+// Codes.  CONV / 32 warps convert the K of every tile and as many others the V, each its share; no warp waits for another
+// one, so that the copies, conversions and stores of some fill the pauses of others.  A lane copies (cp.async) exactly the
+// pieces that it converts, `stages` tiles ahead, and so needs no barrier; in registers they would share the few counters
+// on which a warp waits for loads, and waiting for a tile's would be waiting for the next one's.
+// Slot (tile & 1) of either ring.
+template <int D, int Q, int CONV>
+struct Codes {
+    static constexpr int ROW = Q == IZB_KV_INT8 ? D : D / 2;
+    static constexpr int CHUNKS = ROW / 16, ROWS = 32 / CHUNKS, SHARE = TC_TILE / (CONV / 32), N = SHARE / ROWS;  // tokens copied at a time, a warp's share, copies of it
+    static constexpr int SCALES = Q == IZB_KV_Q4_0 ? N * 32 * 4 : 0;
+    static constexpr int STAGE = N * 32 * 16 + SCALES;                          // bytes of a warp's share of a tile
+    static constexpr __host__ __device__ int bytes(int stages) { return Q == IZB_KV_NONE ? 0 : stages * 2 * (CONV / 32) * STAGE; }
+    // tiles under way: what fits beside query rows and tiles of 16 bits
+    static constexpr __host__ __device__ int stages(bool wide) { return D == 64 ? 3 : wide ? 1 : Q == IZB_KV_INT8 ? 2 : 3; }
+};
+template <int D, int Q, int CONV>
+__device__ __forceinline__ void convert_role(const Params& p, int kv, int warp, int src_row, int kh, int t0, int n_tok, uint32_t ring, uint32_t staging,
+                                             int stages, TcShared& sh) {
+    using C = Codes<D, Q, CONV>;
+    constexpr int LOW = C::CHUNKS / (D / 64);  // pieces of 16 bytes that hold 64 channels
     constexpr int TILE_BYTES = TC_TILE * D * 2;
     const Source& src = p.prefix;
-    const int t = threadIdx.x - 256, lane = t & 31, my_r = t / CHUNKS, my_c = t % CHUNKS;
-    const int n_tiles = (n_tok + TC_TILE - 1) / TC_TILE;
-    const uint32_t stride = static_cast<uint32_t>(p.kv_heads) * ROW;
-    const uint8_t* from[2] = {src.k + kh * ROW + my_c * 16, src.v + kh * ROW + my_c * 16};
-    const float* scales_from[2] = {src.k_scales, src.v_scales};
+    const int lane = threadIdx.x & 31, n_tiles = (n_tok + TC_TILE - 1) / TC_TILE;
+    // The eight lanes of a store phase convert channels of the same 64 for several tokens, whose swizzles differ: eight
+    // different 16-byte columns of the banks.
+    const int my_c = (lane & (LOW - 1)) + (D == 128 ? ((lane >> 3) & 1) * LOW : 0);
+    const int my_r = D == 128 ? (lane & 7) / LOW + (lane >> 4) * (8 / LOW) : lane / LOW;
+    const uint32_t stride = static_cast<uint32_t>(p.kv_heads) * C::ROW;
+    const uint8_t* from = (kv ? src.v : src.k) + kh * C::ROW + my_c * 16;
+    const float* scales_from = (kv ? src.v_scales : src.k_scales) + (Q == IZB_KV_Q4_0 ? kh * (D / 32) + my_c : 0);
     const int* table = src.table + static_cast<long long>(src_row) * src.max_pages;
-    int page = 0, in_page = 0;
-    auto look_up = [&](int tok) {  // threads 0..127: the place of a tile's token, a tile ahead
-        if (t < TC_TILE && tok < n_tok) {
-            const unsigned at = static_cast<unsigned>(t0 + tok), pg = at / static_cast<unsigned>(src.page_size);
-            in_page = static_cast<int>(at - pg * src.page_size);
-            page = table[pg];
+    unsigned long long *full = kv ? sh.v_full : sh.k_full, *empty = kv ? sh.v_empty : sh.k_empty;
+
+    // This lane's token of the tiles to be copied: its page is asked for a tile ahead of that.
+    const int my_tok = warp * C::SHARE + (lane & (C::SHARE - 1));
+    int tok = my_tok, at_page = (t0 + my_tok) / src.page_size, rest = t0 + my_tok - at_page * src.page_size;
+    int page = tok < n_tok ? table[at_page] : 0;
+    float scale[3] = {0.f, 0.f, 0.f};  // Int8: of the page of the lane's token, in turn
+    auto copy = [&](uint32_t to) {
+        const bool in = tok < n_tok;  // what lies past the end becomes zeros with a zero scale
+        const uint32_t my_place = in ? static_cast<uint32_t>(page) * static_cast<uint32_t>(src.page_size) + static_cast<uint32_t>(rest) : ~0u;
+        if (Q == IZB_KV_INT8) {
+            scale[0] = scale[1];
+            scale[1] = scale[2];
+            scale[2] = in ? scales_from[page] : 0.f;
         }
-    };
-    auto publish = [&](int tile) {
-        if (t < TC_TILE) {
-            const bool in = tile * TC_TILE + t < n_tok;
-            sh.place[tile & 3][t] = in ? static_cast<uint32_t>(page) * static_cast<uint32_t>(src.page_size) + static_cast<uint32_t>(in_page) : 0u;
-            if (Q == IZB_KV_INT8) sh.page[tile & 3][t] = in ? static_cast<uint32_t>(page) : 0u;
+#pragma unroll
+        for (int j = 0; j < C::N; ++j) {
+            uint32_t place = __shfl_sync(0xFFFFFFFFu, my_place, j * C::ROWS + my_r);
+            const bool have = place != ~0u;
+            place = have ? place : 0u;
+            cp16(to + j * 512, from + static_cast<uint64_t>(place) * stride, have ? 16 : 0);
+            if constexpr (Q == IZB_KV_Q4_0)
+                cp4(to + C::N * 512 - lane * 12 + j * 128, scales_from + static_cast<uint64_t>(place) * static_cast<uint32_t>(p.kv_heads * (D / 32)), have ? 4 : 0);
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        tok += TC_TILE;
+        at_page += src.step_pages;
+        rest += src.step_rest;
+        if (rest >= src.page_size) { rest -= src.page_size; ++at_page; }
+        page = tok < n_tok ? table[at_page] : 0;
     };
-    // One warp waits for a slot, the barrier behind it holds the others; then all see whether a wait has given up by now.
-    auto slot_free = [&](unsigned long long* empty, int tile, int kv) {
-        if (t < 32 && !wait_phase(&empty[tile & 1], ((tile >> 1) & 1) ^ 1)) {
-            atomicMin(&sh.copy_failed, 2 * tile + kv);
-            sh.failed = 1;
+    const CodeBits<Q> bits;
+    staging += ((kv * (CONV / 32) + warp) * stages) * C::STAGE + lane * 16;
+    for (int i = 0; i < stages; ++i) copy(staging + i * C::STAGE);
+    bool ok = true;
+    uint32_t slot = staging;
+    for (int tile = 0; tile < n_tiles; ++tile) {
+        if (stages == 1) asm volatile("cp.async.wait_group 0;" ::: "memory");
+        else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else asm volatile("cp.async.wait_group 2;" ::: "memory");
+        if (!wait_phase(&empty[tile & 1], ((tile >> 1) & 1) ^ 1)) {
+            ok = false;
+            break;
         }
-    };
-    auto given_up = [&](int tile, int kv) { return *static_cast<volatile int*>(&sh.copy_failed) <= 2 * tile + kv; };
-    auto arrive = [&](unsigned long long* full, int tile) {
+        const uint32_t base = ring + (tile & 1) * TILE_BYTES;
+        uint32_t my_scale = 0;
+        if (Q == IZB_KV_INT8) {
+            const float s = stages == 1 ? scale[2] : stages == 2 ? scale[1] : scale[0];
+            my_scale = pack_bf16x2(s, s);
+        }
+#pragma unroll
+        for (int j = 0; j < C::N; ++j) {
+            const int r = warp * C::SHARE + j * C::ROWS + my_r;
+            const uint4 raw = lds128(slot + j * 512);
+            const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
+            if constexpr (Q == IZB_KV_INT8) {
+                const uint32_t sc2 = __shfl_sync(0xFFFFFFFFu, my_scale, j * C::ROWS + my_r);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t y[4];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        y[2 * i] = hmul2(bits.pair(prmt(x[2 * h + i], 0u, 0x4140)), sc2);
+                        y[2 * i + 1] = hmul2(bits.pair(prmt(x[2 * h + i], 0u, 0x4342)), sc2);
+                    }
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(base + tile_place<D>(r, my_c * 2 + h)), "r"(y[0]), "r"(y[1]),
+                                 "r"(y[2]), "r"(y[3])
+                                 : "memory");
+                }
+            } else {
+                // a word's eight channels in the order 0, 4, 1, 5, 2, 6, 3, 7; so are the query rows, and the outputs are put back
+                const float s = __uint_as_float(lds32(slot + C::N * 512 - lane * 12 + j * 128));
+                uint32_t hi2, lo2;
+                split_scales(s, s, hi2, lo2);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t y[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = q4_value(bits.pair(x[w] >> (4 * e)), hi2, lo2);
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(base + tile_place<D>(r, my_c * 4 + w)), "r"(y[0]), "r"(y[1]),
+                                 "r"(y[2]), "r"(y[3])
+                                 : "memory");
+                }
+            }
+        }
         fence_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&full[tile & 1]));
-    };
-    look_up(t);
-
-    const CodeBits<Q> bits;
-    // the codes and scales of a unit, in registers; each buffer is filled again as soon as it has been converted, two units
-    // ahead of its use
-    uint4 raw[2][N];
-    float sc[2][N];
-    auto load = [&](int tile, int kv) {
-        const int have = n_tok - tile * TC_TILE;
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int r = j * RSTEP + my_r;
-            const uint32_t place = sh.place[tile & 3][r];
-            raw[kv][j] = make_uint4(0u, 0u, 0u, 0u);
-            sc[kv][j] = 0.f;
-            if (r < have) {
-                raw[kv][j] = __ldcs(reinterpret_cast<const uint4*>(from[kv] + static_cast<uint64_t>(place) * stride));
-                if constexpr (Q == IZB_KV_INT8) sc[kv][j] = scales_from[kv][sh.page[tile & 3][r]];
-                else sc[kv][j] = scales_from[kv][static_cast<uint64_t>(place) * static_cast<uint32_t>(p.kv_heads * (D / 32)) + static_cast<uint32_t>(kh * (D / 32) + my_c)];
-            }
-        }
-    };
-    // Two units in registers are 32 KB on the way (Int8, D = 128), a third of what memory needs to run at its rate, so the
-    // lines of tiles further ahead are called into L2.
-    auto call = [&](int tile, int kv) {
-        const int have = n_tok - tile * TC_TILE;
-        if ((my_c * 16) % 128 != 0) return;
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int r = j * RSTEP + my_r;
-            if (r < have) asm volatile("prefetch.global.L2 [%0];" ::"l"(from[kv] + static_cast<uint64_t>(sh.place[tile & 3][r]) * stride));
-        }
-    };
-#pragma unroll
-    for (int i = 0; i < TC_CALLED; ++i) {
-        publish(i);
-        look_up((i + 1) * TC_TILE + t);
+        copy(slot);
+        slot = slot == staging + (stages - 1) * C::STAGE ? staging : slot + C::STAGE;
     }
-    named_bar_sync(2, TC_COPY);
-    load(0, 0);
-    load(0, 1);
-#pragma unroll
-    for (int i = 1; i < TC_CALLED; ++i) {
-        call(i, 0);
-        call(i, 1);
-    }
-    for (int tile = 0; tile < n_tiles; ++tile) {
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-            if (kv == 0) publish(tile + TC_CALLED);  // over a tile that nobody reads any more
-            slot_free(kv ? sh.v_empty : sh.k_empty, tile, kv);
-            named_bar_sync(2, TC_COPY);
-            if (given_up(tile, kv)) return;
-            if (kv == 0) look_up((tile + TC_CALLED + 1) * TC_TILE + t);
-            const uint32_t base = (kv ? v_ring : k_ring) + (tile & 1) * TILE_BYTES;
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int r = j * RSTEP + my_r;
-                const uint32_t x[4] = {raw[kv][j].x, raw[kv][j].y, raw[kv][j].z, raw[kv][j].w};
-                if constexpr (Q == IZB_KV_INT8) {
-                    const uint32_t sc2 = pack_bf16x2(sc[kv][j], sc[kv][j]);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t y[4];
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            y[2 * i] = hmul2(bits.pair(prmt(x[2 * h + i], 0u, 0x4140)), sc2);
-                            y[2 * i + 1] = hmul2(bits.pair(prmt(x[2 * h + i], 0u, 0x4342)), sc2);
-                        }
-                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(base + tile_place<D>(r, my_c * 2 + h)), "r"(y[0]), "r"(y[1]),
-                                     "r"(y[2]), "r"(y[3])
-                                     : "memory");
-                    }
-                } else {
-                    // a word's eight channels in the order 0, 4, 1, 5, 2, 6, 3, 7; so are the query rows, and the outputs are put back
-                    uint32_t hi2, lo2;
-                    split_scales(sc[kv][j], sc[kv][j], hi2, lo2);
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        uint32_t y[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) y[e] = q4_value(bits.pair(x[w] >> (4 * e)), hi2, lo2);
-                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(base + tile_place<D>(r, my_c * 4 + w)), "r"(y[0]), "r"(y[1]),
-                                     "r"(y[2]), "r"(y[3])
-                                     : "memory");
-                    }
-                }
-            }
-            arrive(kv ? sh.v_full : sh.k_full, tile);
-            if (tile + 1 < n_tiles) load(tile + 1, kv);
-            call(tile + TC_CALLED, kv);
-        }
-    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (!ok) sh.failed = 1;
 }
 
-template <int D, int Q>
-__global__ void __launch_bounds__(tc_threads(Q), 1)
+template <int D, int Q, int CONV>
+__global__ void __launch_bounds__(Roles<Q, CONV>::THREADS, 1)
     shared_prefix_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Maps maps, int wide) {
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ TcShared sh;
     constexpr int TILE_BYTES = TC_TILE * D * 2, Q_BYTES = 128 * D * 2;
-    constexpr bool CODES = Q != IZB_KV_NONE;
-    constexpr int ISSUE_WARP = CODES ? 16 : 9;
+    using R = Roles<Q, CONV>;
+    constexpr bool CODES = R::CODES;
+    constexpr int ISSUE_WARP = R::ISSUE_WARP;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     // ---- the item ----
@@ -361,17 +353,17 @@ __global__ void __launch_bounds__(tc_threads(Q), 1)
     const uint32_t sq = smem_u32(smem), k_ring = sq + (wide ? 2 : 1) * Q_BYTES, v_ring = k_ring + 2 * TILE_BYTES;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_u32(&sh.k_full[i]), CODES ? TC_COPY / 32 : 1);
-            mbar_init(smem_u32(&sh.v_full[i]), CODES ? TC_COPY / 32 : 1);
+            mbar_init(smem_u32(&sh.k_full[i]), CODES ? CONV / 32 : 1);
+            mbar_init(smem_u32(&sh.v_full[i]), CODES ? CONV / 32 : 1);
             mbar_init(smem_u32(&sh.k_empty[i]), 1);
             mbar_init(smem_u32(&sh.v_empty[i]), 1);
             mbar_init(smem_u32(&sh.s_full[i]), 1);
             mbar_init(smem_u32(&sh.p_full[i][0]), 4);
             mbar_init(smem_u32(&sh.p_full[i][1]), 4);
-            mbar_init(smem_u32(&sh.pv_done[i]), 1);
+            mbar_init(smem_u32(&sh.pv_done[i][0]), 1);
+            mbar_init(smem_u32(&sh.pv_done[i][1]), 1);
         }
         mbar_init(smem_u32(&sh.q_full), 8);
-        sh.copy_failed = INT_MAX;
         sh.failed = 0;
         mbar_fence_init();
     }
@@ -385,17 +377,19 @@ __global__ void __launch_bounds__(tc_threads(Q), 1)
     constexpr uint32_t tmem = 0;
 
     // Each role ends by itself: code shared behind it would have to fit the smallest of their register counts.
-    if (CODES ? (warp >= 8 && warp < 16) : (warp >= 8 && warp != ISSUE_WARP)) {
+    if (CODES ? (warp >= 8 && warp < ISSUE_WARP) : (warp >= 8 && warp != ISSUE_WARP)) {
         if constexpr (CODES) {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TC_COPY_REGS));
-            convert_role<D, Q>(p, group, kh, t0, n_tok, k_ring, v_ring, sh);
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::COPY));
+            const int kv = (warp - 8) / (CONV / 32);
+            convert_role<D, Q, CONV>(p, kv, (warp - 8) % (CONV / 32), group, kh, t0, n_tok, kv ? v_ring : k_ring, v_ring + 2 * TILE_BYTES,
+                               Codes<D, Q, CONV>::stages(wide), sh);
         } else if (warp == 8) {
             fetch_role<D>(p, maps, group, kh, t0, n_tok, k_ring, v_ring, sh);
         }
         __syncthreads();
     } else if (warp >= 8) {
         // ---------------- products ----------------
-        if constexpr (CODES) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TC_ISSUE_REGS));
+        if constexpr (CODES) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::ISSUE));
         if (warp == ISSUE_WARP) {
             tc_alloc(smem_u32(&sh.tmem), 512);
             // The whole warp walks the schedule, so that addresses and descriptors stay in uniform registers, and one lane
@@ -437,7 +431,7 @@ __global__ void __launch_bounds__(tc_threads(Q), 1)
                         for (int k = half * 4; k < half * 4 + 4; ++k)
                             mma_ts(256 + v * 128, v * 128 + k * 8, b + static_cast<uint64_t>(k * (2048 >> 4)), o_idesc, nth != 0 || k != 0);
                         if (half && last_use) tc_commit(smem_u32(&sh.v_empty[tile & 1]));
-                        if (half) tc_commit(smem_u32(&sh.pv_done[v]));
+                        tc_commit(smem_u32(&sh.pv_done[v][half]));
                     }
                     __syncwarp();
                 }
@@ -469,7 +463,10 @@ __global__ void __launch_bounds__(tc_threads(Q), 1)
         }
     } else {
         // ---------------- weights ----------------
-        if constexpr (CODES) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TC_WEIGHT_REGS));
+        if constexpr (CODES) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R::WEIGHTS));
+        // With at most 32 (64) rows the second set has them once more from lane 32 (64) on, so that the two sets' weights are
+        // computed on different quarters of the SM.
+        const int twin = wide || n_rows > 64 ? 128 : n_rows > 32 ? 64 : 32;
         // the query rows, K-major, all of a thread's 16-byte pieces under way at once
         {
             constexpr int C = D / 8, STEP = 256 / C, B = CODES ? 8 : 16;
@@ -478,9 +475,9 @@ __global__ void __launch_bounds__(tc_threads(Q), 1)
                 uint4 x[B];
 #pragma unroll
                 for (int j = 0; j < B; ++j) {
-                    const int r = r0 + j * STEP, at = row0 + r;
+                    const int r = r0 + j * STEP, nth = !wide && r >= twin ? r - twin : r, at = row0 + nth;
                     x[j] = make_uint4(0u, 0u, 0u, 0u);
-                    if (r < n_rows) {
+                    if (nth < n_rows) {
                         const int s = at / p.g, h = at - s * p.g;
                         x[j] = *reinterpret_cast<const uint4*>(p.q + (seq0 + s) * p.ld_q + static_cast<long long>(kh * p.g + h) * D + c * 8);
                     }
@@ -500,15 +497,15 @@ __global__ void __launch_bounds__(tc_threads(Q), 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sh.q_full));
         }
-        const int v = warp >> 2, row = (warp & 3) * 32 + lane;               // lane of tensor memory
-        const int first = (wide ? v * 128 : 0) + (warp & 3) * 32;             // this warp's first row of the block
+        const int v = warp >> 2;
+        const int first = (wide ? v * 128 : -v * (twin & 127)) + (warp & 3) * 32;  // this warp's first row of the block
         const int mine = wide ? n_tiles : (n_tiles + 1 - v) / 2;              // tiles of this set
         const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t t_s = t_lane + v * 128, t_o = t_lane + 256 + v * 128;
-        const bool live = first < n_rows;                                      // else the warp only keeps the barriers going
+        const bool live = first >= 0 && first < n_rows;                        // else the warp only keeps the barriers going
         float m = -INFINITY, l = 0.f;
         bool ok = true;
-        for (int n = 0; n < mine; ++n) {
+        for (int n = 0; n < mine && ok; ++n) {
             const int tile = wide ? n : 2 * n + v;
             if (!wait_phase(&sh.s_full[v], n & 1)) {
                 ok = false;
@@ -516,63 +513,57 @@ __global__ void __launch_bounds__(tc_threads(Q), 1)
             }
             tc_fence_after();
             const int left = n_tok - tile * TC_TILE;
-            auto masked = [&](float(&s)[64], int c0) {
+            auto largest = [&](float(&x)[64], int c0) {  // of 64 scores; those past the end become -inf
                 if (left < c0 + 64) {
 #pragma unroll
                     for (int i = 0; i < 64; ++i)
-                        if (c0 + i >= left) s[i] = -INFINITY;
+                        if (c0 + i >= left) x[i] = -INFINITY;
                 }
-            };
-            auto largest = [&](const float(&s)[64]) {
                 float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int i = 0; i < 64; i += 8)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) t[k] = fmaxf(t[k], fmaxf(s[i + 2 * k], s[i + 2 * k + 1]));
+                    for (int k = 0; k < 4; ++k) t[k] = fmaxf(t[k], fmaxf(x[i + 2 * k], x[i + 2 * k + 1]));
                 return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
             };
-            float s[2][64];  // codes: the halves one after the other, read twice
-            if (live) {
-                float top;
+            float s[2][64];  // bf16 pages: both halves are read at once; codes, with fewer registers: one after the other
+            if (!CODES && live) {
                 tc_ld_32x64(t_s, s[0]);
-                if constexpr (!CODES) tc_ld_32x64(t_s + 64, s[1]);
-                masked(s[0], 0);
-                top = largest(s[0]);
-                if constexpr (CODES) tc_ld_32x64(t_s + 64, s[0]);
-                masked(s[CODES ? 0 : 1], 64);
-                top = fmaxf(top, largest(s[CODES ? 0 : 1]));
-                // The reference point of a row follows its maximum only when that has grown by 2^8 in weight (not-less: also for
-                // the first maximum): weights up to 2^8 are as exact as weights up to 1, and the output is seldom rescaled.
-                if (__any_sync(0xFFFFFFFFu, !(top <= m + p.margin))) {
-                    const float to = fmaxf(m, top), f = m == -INFINITY ? 0.f : ex2((m - to) * p.scale_log2);
-                    m = to;
-                    l *= f;
-                    if (n > 0) {
-                        if (!wait_phase(&sh.pv_done[v], (n - 1) & 1)) {  // the set's output so far is complete
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-#pragma unroll 1
-                        for (int c = 0; c < D / 8; ++c) {
-                            uint32_t x[8];
-                            tc_ld_32x8(t_o + c * 8, x);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
-                            tc_st_32x8(t_o + c * 8, x);
-                        }
-                    }
-                }
+                tc_ld_32x64(t_s + 64, s[1]);
             }
-            const float u = m == -INFINITY ? 0.f : m * p.scale_log2;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 if (live) {
                     float(&x)[64] = s[CODES ? 0 : half];
-                    if constexpr (CODES) {
-                        tc_ld_32x64(t_s + half * 64, x);
-                        masked(x, half * 64);
+                    if constexpr (CODES) tc_ld_32x64(t_s + half * 64, x);
+                    float top = -INFINITY;
+                    if constexpr (CODES) top = largest(x, half * 64);
+                    else if (half == 0) top = fmaxf(largest(s[0], 0), largest(s[1], 64));
+                    // The reference point of a row follows its maximum only when that has grown by 2^8 in weight (not-less: also for
+                    // the first maximum): weights up to 2^8 are as exact as weights up to 1, and the output is seldom rescaled.  With
+                    // codes it may do so for either half of a tile: the scores are read once, and the first half's product does not wait
+                    // for the second's maximum.
+                    if ((CODES || half == 0) && __any_sync(0xFFFFFFFFu, !(top <= m + p.margin))) {
+                        const float to = fmaxf(m, top), f = m == -INFINITY ? 0.f : ex2((m - to) * p.scale_log2);
+                        m = to;
+                        l *= f;
+                        if (n > 0 || half > 0) {
+                            if (!wait_phase(&sh.pv_done[v][half ^ 1], (n - 1 + half) & 1)) {  // the set's output so far is complete
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < D / 8; ++c) {
+                                uint32_t y[8];
+                                tc_ld_32x8(t_o + c * 8, y);
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+                                tc_st_32x8(t_o + c * 8, y);
+                            }
+                        }
                     }
+                    const float u = m == -INFINITY ? 0.f : m * p.scale_log2;
                     // weights over scores that have been read: 64 become 32 columns
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -594,7 +585,7 @@ __global__ void __launch_bounds__(tc_threads(Q), 1)
                 if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[v][half]));
             }
         }
-        if (ok && mine > 0 && !wait_phase(&sh.pv_done[v], (mine - 1) & 1)) ok = false;
+        if (ok && mine > 0 && !wait_phase(&sh.pv_done[v][1], (mine - 1) & 1)) ok = false;
         if (!ok) sh.failed = 1;
         tc_fence_after();
         // Both sets are complete: the rows go through shared memory, where the tiles were, so that a row is written as one
@@ -603,7 +594,7 @@ __global__ void __launch_bounds__(tc_threads(Q), 1)
         constexpr int LD = D + 4;
         float* stage = reinterpret_cast<float*>(smem);
         if (live && mine > 0) {
-            float* dst = stage + (v * 128 + row) * LD;
+            float* dst = stage + (wide ? first + lane : v * 128 + first + lane) * LD;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
                 float o[32];
@@ -620,7 +611,7 @@ __global__ void __launch_bounds__(tc_threads(Q), 1)
                 }
             }
         }
-        sh.ml[v][row] = make_float2(m, l);
+        if (live) sh.ml[v][(first & 127) + lane] = make_float2(m, l);
         named_bar_sync(3, 256);
         const int chunks = p.prefix.n_chunks + p.own.n_chunks;
         constexpr int LANES = D / 4, RW = 32 / LANES;  // lanes of a row, rows of a warp at a time
@@ -645,17 +636,18 @@ __global__ void __launch_bounds__(tc_threads(Q), 1)
     }
 }
 
-template <int D, int Q>
+template <int D, int Q, int CONV>
 int launch(izb_ctx* ctx, cudaStream_t s, const Params& p, int64_t items, bool wide) {
-    auto kern = shared_prefix_tc_kernel<D, Q>;
+    auto kern = shared_prefix_tc_kernel<D, Q, CONV>;
     constexpr int RING = 4 * TC_TILE * D * 2, Q_BYTES = 128 * D * 2;
+    auto smem = [](bool w) { return (w ? 2 : 1) * Q_BYTES + RING + Codes<D, Q, CONV>::bytes(Codes<D, Q, CONV>::stages(w)); };
     static std::atomic<bool> ready[IZB_MAX_DEVICES];
     if (!ready[ctx->device].load(std::memory_order_relaxed)) {
         cudaFuncAttributes attr;
         IZB_CUDA_TRY(cudaFuncGetAttributes(&attr, kern));
         // the weight warps would wait for registers nobody has
-        if (Q != IZB_KV_NONE && attr.numRegs < TC_LAUNCH_REGS) return IZB_ERR_LAUNCH;
-        IZB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * Q_BYTES + RING));
+        if (Q != IZB_KV_NONE && attr.numRegs < Roles<Q, CONV>::LAUNCH) return IZB_ERR_LAUNCH;
+        IZB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem(false) > smem(true) ? smem(false) : smem(true)));
         ready[ctx->device].store(true, std::memory_order_relaxed);
     }
     Maps maps = {};
@@ -672,10 +664,20 @@ int launch(izb_ctx* ctx, cudaStream_t s, const Params& p, int64_t items, bool wi
             if (rc != IZB_OK) return rc;
         }
     }
-    IZB_CUDA_TRY(launch_chained(ctx, kern, dim3(static_cast<unsigned>(items)), dim3(tc_threads(Q)), static_cast<size_t>((wide ? 2 : 1) * Q_BYTES + RING), s, p,
+    IZB_CUDA_TRY(launch_chained(ctx, kern, dim3(static_cast<unsigned>(items)), dim3(Roles<Q, CONV>::THREADS), static_cast<size_t>(smem(wide)), s, p,
                                 maps, wide ? 1 : 0));
     ctx->launches.fetch_add(1, std::memory_order_relaxed);
     return IZB_OK;
+}
+
+// Converting warps: eight, and sixteen for Int8 under up to 128 rows.  Sixteen convert a tile faster and take issue slots
+// from the weights.  D = 128, 8 x 32 heads per KV head's prefix: Int8 4,099 tokens x 32 groups 111 us with sixteen, 125 with
+// eight; Q4_0 9,001 tokens x 32 groups 156 and 151; Int8 under 256 rows 195 and 184.
+template <int D>
+int launch_dim(izb_ctx* ctx, cudaStream_t s, const Params& p, int64_t items, bool wide) {
+    if (p.prefix.quant == IZB_KV_NONE) return launch<D, IZB_KV_NONE, 128>(ctx, s, p, items, wide);
+    if (p.prefix.quant == IZB_KV_Q4_0) return launch<D, IZB_KV_Q4_0, 128>(ctx, s, p, items, wide);
+    return wide ? launch<D, IZB_KV_INT8, 128>(ctx, s, p, items, wide) : launch<D, IZB_KV_INT8, 256>(ctx, s, p, items, wide);
 }
 
 }  // namespace
@@ -683,12 +685,7 @@ int launch(izb_ctx* ctx, cudaStream_t s, const Params& p, int64_t items, bool wi
 int launch_prefix_tc(izb_ctx* ctx, cudaStream_t s, const Params& p, int head_dim, int64_t groups) {
     const bool wide = static_cast<int64_t>(p.seqs) * p.g > TC_ROWS;
     const int64_t items = groups * p.prefix.n_chunks * p.kv_heads * p.row_blocks;
-    const int q = p.prefix.quant;
-    if (head_dim == 128)
-        return q == IZB_KV_NONE ? launch<128, IZB_KV_NONE>(ctx, s, p, items, wide) : q == IZB_KV_INT8 ? launch<128, IZB_KV_INT8>(ctx, s, p, items, wide)
-                                                                                                       : launch<128, IZB_KV_Q4_0>(ctx, s, p, items, wide);
-    return q == IZB_KV_NONE ? launch<64, IZB_KV_NONE>(ctx, s, p, items, wide) : q == IZB_KV_INT8 ? launch<64, IZB_KV_INT8>(ctx, s, p, items, wide)
-                                                                                                  : launch<64, IZB_KV_Q4_0>(ctx, s, p, items, wide);
+    return head_dim == 128 ? launch_dim<128>(ctx, s, p, items, wide) : launch_dim<64>(ctx, s, p, items, wide);
 }
 
 }  // namespace shared_prefix

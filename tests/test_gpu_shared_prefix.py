@@ -319,3 +319,28 @@ def test_two_graphs_share_a_workspace(cuda):
     torch.cuda.synchronize()
     for _, _, _, _, want, out in sides:
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("quant", ["none", "int8", "q4_0"])
+@pytest.mark.parametrize("seqs,heads,slens", [(3, 8, [70, 0, 1]), (11, 8, [70, 0, 1] * 3 + [64, 128]), (11, 8, [900] + [0] * 10), (4, 16, [5] * 4)])
+def test_rows_of_any_stride_and_address(cuda, quant, seqs, heads, slens):
+    """Results two bytes off a word, rows an odd number of elements apart, what lies between them left as it was; few and
+    many rows, own tokens in one item and in several, in the last launch and before it."""
+    import ctypes as C
+
+    from izwi_b200 import _lib as L
+    from izwi_b200 import ops, paged
+    rng = np.random.default_rng(len(slens))
+    prefix, own = Pool(rng, cuda, [1500], 2, 128, 16, quant), Pool(rng, cuda, slens, 2, 128, 16, quant)
+    q = torch.from_numpy(rng.normal(0, 1, (seqs, heads, 128)).astype(np.float32)).to(cuda).to(torch.bfloat16)
+    want = paged.shared_prefix_attention(q, prefix.cache, own.cache).reshape(seqs, -1)
+    p, o, lib, ctx = prefix.cache, own.cache, L.lib(), ops.Context.get(0)
+    ld = heads * 128 + 3
+    room = torch.full((seqs * ld + 1,), 7.0, device=cuda, dtype=torch.bfloat16)
+    need = lib.izb_shared_prefix_decode_gqa_attention_workspace_bytes(ctx.handle, 1, seqs, heads, 2, 128, p.max_tokens, o.max_tokens)
+    ws = torch.empty(need, device=cuda, dtype=torch.uint8)
+    L.check(lib.izb_shared_prefix_decode_gqa_attention(
+        ctx.handle, C.c_void_p(torch.cuda.current_stream().cuda_stream), q.data_ptr(), C.byref(p._desc), p.seq_lens.data_ptr(), C.byref(o._desc),
+        o.seq_lens.data_ptr(), room.data_ptr() + 2, 1, seqs, heads, p.max_tokens, o.max_tokens, heads * 128, ld, 128 ** -0.5, ws.data_ptr(), need), "call")
+    got = room[1:].reshape(seqs, ld)
+    assert torch.equal(got[:, :-3], want) and (got[:, -3:] == 7).all() and room[0] == 7
