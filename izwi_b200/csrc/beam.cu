@@ -203,6 +203,7 @@ struct SelectParams {
     u64* tile_top;    // [rows][tiles][n_out]: key_of(value) << 32 | ~index, descending; 0: none
     long long ld;
     int vocab, beams, tiles, n_out, eos;
+    int* status;
 };
 
 // A row whose beam is not alive or is finished is not read.
@@ -210,44 +211,62 @@ __device__ __forceinline__ bool row_counts(const SelectParams& p, int row) {
     return isfinite(p.scores[row]) && !(p.finished && p.finished[row]);
 }
 
-// One CTA per tile of BS_THREADS * NV 16-byte vectors of a row, copied asynchronously into shared memory, where three
-// short loops look at it (maximum, sum, candidates); a thread works on the vectors it copied.  (Held in registers with
+// One CTA per tile of BS_THREADS * NV 16-byte vectors of a row, copied into shared memory, where three
+// short loops look at it (maximum, sum, candidates); a thread works on every BS_THREADS-th vector.  (Held in registers with
 // everything unrolled, the tile made straight-line code that each CTA ran once, at the speed of instruction fetch: 144 us
-// for 32 x 8 rows of 151936 bf16 logits.)  Rows may start anywhere: vectors are cut on 16-byte boundaries of memory
-// and the ragged ends are read element by element.  Only finite logits count.
+// for 32 x 8 rows of 151936 bf16 logits.)  Rows may start anywhere: vectors are cut on 16-byte boundaries of memory; a tile
+// inside its row is one bulk copy, and the ragged ends are read element by element.  Only finite logits count.
 template <typename T, int NV>
 __global__ void __launch_bounds__(BS_THREADS) beam_tile_kernel(const __grid_constant__ SelectParams p) {
     constexpr int V = 16 / sizeof(T);
     constexpr float LOG2E = 1.4426950408889634f;
-    __shared__ uint4 tile_s[BS_THREADS * NV];
+    __shared__ __align__(128) uint4 tile_s[BS_THREADS * NV];
     __shared__ Pool pool;
     __shared__ uint32_t slots[BS_WARPS];
     __shared__ float wm[BS_WARPS], wl[BS_WARPS];
+    __shared__ unsigned long long landed;
+    __shared__ int abort_flag;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        izb::mbar_init(izb::smem_u32(&landed), 1);
+        izb::mbar_fence_init();
+        pool.count = 0;
+        abort_flag = 0;
+    }
+    __syncthreads();
     izb::pdl_launch_dependents();
     izb::pdl_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row = blockIdx.x / p.tiles, tile = blockIdx.x - row * p.tiles;
     if (!row_counts(p, row)) return;
     const T* base = static_cast<const T*>(p.logits) + static_cast<long long>(row) * p.ld;
     const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
     const int first = tile * (BS_THREADS * NV) + tid;
     uint4* mine = tile_s + tid;  // vector i at mine[i * BS_THREADS]
-    if (tid == 0) pool.count = 0;
 
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const long long e0 = static_cast<long long>(first + i * BS_THREADS) * V - skew;
-        if (e0 >= 0 && e0 + V <= p.vocab) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(izb::smem_u32(mine + i * BS_THREADS)), "l"(base + e0) : "memory");
-        } else {
-            T* w = reinterpret_cast<T*>(mine + i * BS_THREADS);
-            for (int k = 0; k < V; ++k) {
-                const long long e = e0 + k;
-                w[k] = e >= 0 && e < p.vocab ? base[e] : static_cast<T>(-INFINITY);
+    const long long tile0 = static_cast<long long>(tile) * (BS_THREADS * NV * V) - skew;
+    bool ok = true;
+    if (tile0 >= 0 && tile0 + BS_THREADS * NV * V <= p.vocab) {
+        if (tid == 0) {
+            izb::mbar_expect_tx(izb::smem_u32(&landed), sizeof(tile_s));
+            izb::bulk_g2s(izb::smem_u32(tile_s), base + tile0, sizeof(tile_s), izb::smem_u32(&landed));
+        }
+        ok = izb::mbar_wait_bounded(izb::smem_u32(&landed), 0, &abort_flag);
+    } else {
+#pragma unroll 1
+        for (int i = 0; i < NV; ++i) {
+            const long long e0 = static_cast<long long>(first + i * BS_THREADS) * V - skew;
+            if (e0 >= 0 && e0 + V <= p.vocab) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(izb::smem_u32(mine + i * BS_THREADS)), "l"(base + e0) : "memory");
+            } else {
+                T* w = reinterpret_cast<T*>(mine + i * BS_THREADS);
+                for (int k = 0; k < V; ++k) {
+                    const long long e = e0 + k;
+                    w[k] = e >= 0 && e < p.vocab ? base[e] : static_cast<T>(-INFINITY);
+                }
             }
         }
+        asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
     }
-    asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
 
     float mx = -INFINITY, vm[NV];  // the largest of each vector
 #pragma unroll
@@ -269,12 +288,32 @@ __global__ void __launch_bounds__(BS_THREADS) beam_tile_kernel(const __grid_cons
             mx = fmaxf(mx, vm[i]);
         }
     }
-    // every thread's largest value bounds the tile's n_out largest; ties are left to collect()
-    const u64 bound = block_bound(mx > -INFINITY ? key_of(mx) : 0u, p.n_out, slots);
-
     float top = mx;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    if (lane == 0) wm[warp] = top;
+    if (!__syncthreads_and(ok)) {
+        if (tid == 0) atomicExch(p.status, 1);
+        if (!ok) {  // the copy under way lands in memory of this CTA
+            abort_flag = 0;
+            izb::mbar_wait_bounded(izb::smem_u32(&landed), 0, &abort_flag);
+        }
+        return;
+    }
+    // A bound of the tile's n_out largest; ties are left to collect().  With up to as many as there are warps, the n_out-th
+    // largest of the warps' maxima (n_out warps have a value that is no smaller), else one from every thread's largest.
+    u64 bound;
+    if (p.n_out <= BS_WARPS) {
+        const float v = wm[lane % BS_WARPS];
+        int rank = 0;
+#pragma unroll
+        for (int j = 0; j < BS_WARPS; ++j) rank += wm[j] > v || (wm[j] == v && j < lane % BS_WARPS);
+        const float b = __shfl_sync(0xFFFFFFFFu, v, __ffs(__ballot_sync(0xFFFFFFFFu, rank == p.n_out - 1)) - 1);
+        bound = b > -INFINITY ? static_cast<u64>(key_of(b)) << 32 : 0ull;
+    } else {
+        bound = block_bound(mx > -INFINITY ? key_of(mx) : 0u, p.n_out, slots);
+    }
+
     float sum = 0.f;
     if (top > -INFINITY) {
         const float shift = top * LOG2E;
@@ -300,10 +339,7 @@ __global__ void __launch_bounds__(BS_THREADS) beam_tile_kernel(const __grid_cons
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    if (lane == 0) {
-        wm[warp] = top;
-        wl[warp] = sum;
-    }
+    if (lane == 0) wl[warp] = sum;
     const int n = collect(pool, bound, p.n_out, [&](u64 bk, uint32_t bi) {
         const float floor_v = bk >> 32 ? value_of(static_cast<uint32_t>(bk >> 32)) : -INFINITY;
         // which vectors hold a candidate, then only those, element by element
@@ -758,6 +794,7 @@ int32_t izb_beam_select(izb_ctx* ctx, izb_stream stream, const void* logits, int
     p.tiles = static_cast<int>(pl.tiles);
     p.n_out = n_out;
     p.eos = eos;
+    p.status = ctx->d_status;
     izb::DeviceGuard guard(ctx->device);
     if (!guard.ok) return IZB_ERR_LAUNCH;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
