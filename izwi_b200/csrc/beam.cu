@@ -20,7 +20,7 @@ constexpr int BS_THREADS = 256;
 constexpr int BS_WARPS = BS_THREADS / 32;
 constexpr int BS_MAX_BEAMS = 32;
 constexpr int BS_MAX_OUT = 64;
-constexpr int BS_CAP = 1024;  // candidates kept in shared memory at a time
+constexpr int BS_TILE_CAP = 512, BS_CAP = 1024;  // candidates of a tile, of a group kept in shared memory at a time
 
 using u64 = unsigned long long;
 
@@ -28,6 +28,20 @@ __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
+}
+// two multiply-adds, two additions in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
 }
 // larger value <-> larger key, -0 as +0
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -57,64 +71,67 @@ __device__ __forceinline__ uint32_t warp_kth(uint32_t x, int k) {
     return __shfl_sync(0xFFFFFFFFu, x, k - 1);
 }
 
-// A bound below which none of the k largest candidates can lie, from the upper 32 bits of every thread's largest key:
-// the k-th largest lane of any warp is such a bound (k <= 32), for more the smaller bound of two warps that give half
-// of them each.  `slots` holds one value per warp; every thread returns the largest bound.
-__device__ __forceinline__ u64 block_bound(uint32_t mine, int k, uint32_t* slots) {
+// A bound below which none of the k <= 64 largest candidates can lie, from the upper 32 bits of every thread's largest
+// key.  The k-th largest of the maxima of 32 groups of threads is one (k groups hold a candidate that is no smaller), and a
+// close one when k is well below 32 (22 candidates lie above the median of 32 maxima).
+// So the block is cut into 32 groups, or for larger k into two or four sets of 32 smaller ones, and each set answers for its
+// share of k.  Every thread returns the bound.
+__device__ __forceinline__ u64 block_bound(uint32_t mine, int k, uint32_t (*all)[32], uint32_t (&set)[4]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t w = warp_kth(mine, k <= 32 ? k : (k + 1) / 2);
-    if (lane == 0) slots[warp] = w;
+    const int sets = k <= 20 ? 1 : k <= 40 ? 2 : 4, share = (k + sets - 1) / sets;
+    all[warp][lane] = mine;  // group: the threads of a lane, of every (second, fourth) warp
     __syncthreads();
-    uint32_t bound = 0;
-#pragma unroll
-    for (int i = 0; i < BS_WARPS; i += 2) {
-        const uint32_t a = slots[i], b = slots[i + 1];
-        bound = max(bound, k <= 32 ? max(a, b) : min(a, b));
+    if (warp < sets) {
+        uint32_t v = 0;
+        for (int w = warp; w < BS_WARPS; w += sets) v = max(v, all[w][lane]);
+        v = warp_kth(v, share);
+        if (lane == 0) set[warp] = v;
     }
+    __syncthreads();
+    uint32_t bound = set[0];
+    for (int i = 1; i < sets; ++i) bound = min(bound, set[i]);
     return static_cast<u64>(bound) << 32;
 }
 
-// Candidates in shared memory: a key and, among equal keys, the lower index first.
+// Candidates in shared memory: a key and, among equal keys, the lower index first.  PACKED: keys are different and say it all.
+template <int N, bool PACKED>
 struct Pool {
-    u64 key[BS_CAP];
-    uint32_t idx[BS_CAP];
+    static constexpr int CAP = N;
+    u64 key[N];
+    uint32_t idx[PACKED ? 1 : N];
     unsigned count;
-};
-__device__ __forceinline__ bool before(u64 ka, uint32_t ia, u64 kb, uint32_t ib) { return ka > kb || (ka == kb && ia < ib); }
-
-__device__ __forceinline__ void pool_add(Pool& p, u64 key, uint32_t idx) {
-    const unsigned at = atomicAdd(&p.count, 1u);
-    if (at < BS_CAP) {
-        p.key[at] = key;
-        p.idx[at] = idx;
+    __device__ __forceinline__ static bool before(u64 ka, uint32_t ia, u64 kb, uint32_t ib) { return ka > kb || (!PACKED && ka == kb && ia < ib); }
+    __device__ __forceinline__ uint32_t index(int i) const { return PACKED ? 0u : idx[PACKED ? 0 : i]; }
+    __device__ __forceinline__ void put(int i, u64 k, uint32_t x) {
+        key[i] = k;
+        if (!PACKED) idx[PACKED ? 0 : i] = x;
     }
-}
-// Descending order over the first n entries (n <= BS_CAP).  Up to one entry per thread: each counts the entries in
+    __device__ __forceinline__ void add(u64 k, uint32_t x) {
+        const unsigned at = atomicAdd(&count, 1u);
+        if (at < N) put(at, k, x);
+    }
+};
+// Descending order over the first n entries (n <= CAP).  Up to one entry per thread: each counts the entries in
 // front of it (n broadcast reads, no barrier between them); more: bitonic exchange over the next power of two.
-__device__ void pool_sort(Pool& p, int n) {
+template <typename P>
+__device__ void pool_sort(P& p, int n) {
     if (n <= BS_THREADS) {
         const int i = threadIdx.x;
         const u64 key = i < n ? p.key[i] : 0;
-        const uint32_t idx = i < n ? p.idx[i] : 0;
+        const uint32_t idx = i < n ? p.index(i) : 0;
         int rank = 0;
         if (i < n) {
 #pragma unroll 4
-            for (int j = 0; j < n; ++j) rank += before(p.key[j], p.idx[j], key, idx);
+            for (int j = 0; j < n; ++j) rank += P::before(p.key[j], p.index(j), key, idx);
         }
         __syncthreads();
-        if (i < n) {
-            p.key[rank] = key;
-            p.idx[rank] = idx;
-        }
+        if (i < n) p.put(rank, key, idx);
         __syncthreads();
         return;
     }
     int size = 2 * BS_THREADS;
     while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += BS_THREADS) {
-        p.key[i] = 0;
-        p.idx[i] = 0xFFFFFFFFu;
-    }
+    for (int i = n + threadIdx.x; i < size; i += BS_THREADS) p.put(i, 0, 0xFFFFFFFFu);
     __syncthreads();
     for (int block = 2; block <= size; block <<= 1)
         for (int step = block >> 1; step > 0; step >>= 1) {
@@ -122,10 +139,10 @@ __device__ void pool_sort(Pool& p, int n) {
                 const int a = 2 * i - (i & (step - 1)), b = a + step;
                 const bool down = (a & block) == 0;
                 const u64 ka = p.key[a], kb = p.key[b];
-                const uint32_t ia = p.idx[a], ib = p.idx[b];
-                if (before(kb, ib, ka, ia) == down) {
-                    p.key[a] = kb; p.idx[a] = ib;
-                    p.key[b] = ka; p.idx[b] = ia;
+                const uint32_t ia = p.index(a), ib = p.index(b);
+                if (P::before(kb, ib, ka, ia) == down) {
+                    p.put(a, kb, ib);
+                    p.put(b, ka, ia);
                 }
             }
             __syncthreads();
@@ -134,20 +151,20 @@ __device__ void pool_sort(Pool& p, int n) {
 
 // Fills the pool with every candidate not behind (bound_key, bound_idx); when they outgrow it, the k-th of those it
 // caught is a tighter bound (any k candidates bound the k largest), and the scan is repeated: each repetition drops
-// at least BS_CAP - k candidates for good.  Then sorts.  Returns the number of sorted entries, at least the k
+// at least CAP - k candidates for good.  Then sorts.  Returns the number of sorted entries, at least the k
 // largest if there are that many.  `scan(key, idx)` calls add for every candidate not behind the bound.  The pool's
 // count is zero, and every thread knows it, on the first entry.
-template <typename Scan>
-__device__ int collect(Pool& p, u64 bound_key, int k, Scan scan) {
+template <typename P, typename Scan>
+__device__ int collect(P& p, u64 bound_key, int k, Scan scan) {
     uint32_t bound_idx = 0xFFFFFFFFu;
     for (;;) {
         scan(bound_key, bound_idx);
         __syncthreads();
         const unsigned n = p.count;
-        pool_sort(p, n < BS_CAP ? n : BS_CAP);
-        if (n <= BS_CAP) return static_cast<int>(n);
+        pool_sort(p, n < P::CAP ? n : P::CAP);
+        if (n <= P::CAP) return static_cast<int>(n);
         bound_key = p.key[k - 1];
-        bound_idx = p.idx[k - 1];
+        bound_idx = p.index(k - 1);
         if (threadIdx.x == 0) p.count = 0;
         __syncthreads();
     }
@@ -217,12 +234,12 @@ __device__ __forceinline__ bool row_counts(const SelectParams& p, int row) {
 // for 32 x 8 rows of 151936 bf16 logits.)  Rows may start anywhere: vectors are cut on 16-byte boundaries of memory; a tile
 // inside its row is one bulk copy, and the ragged ends are read element by element.  Only finite logits count.
 template <typename T, int NV>
-__global__ void __launch_bounds__(BS_THREADS) beam_tile_kernel(const __grid_constant__ SelectParams p) {
+__global__ void __launch_bounds__(BS_THREADS, NV == 8 ? 6 : 8) beam_tile_kernel(const __grid_constant__ SelectParams p) {
     constexpr int V = 16 / sizeof(T);
     constexpr float LOG2E = 1.4426950408889634f;
     __shared__ __align__(128) uint4 tile_s[BS_THREADS * NV];
-    __shared__ Pool pool;
-    __shared__ uint32_t slots[BS_WARPS];
+    __shared__ Pool<BS_TILE_CAP, true> pool;  // key_of(value) << 32 | ~index
+    __shared__ uint32_t sets[4];
     __shared__ float wm[BS_WARPS], wl[BS_WARPS];
     __shared__ unsigned long long landed;
     __shared__ int abort_flag;
@@ -311,20 +328,24 @@ __global__ void __launch_bounds__(BS_THREADS) beam_tile_kernel(const __grid_cons
         const float b = __shfl_sync(0xFFFFFFFFu, v, __ffs(__ballot_sync(0xFFFFFFFFu, rank == p.n_out - 1)) - 1);
         bound = b > -INFINITY ? static_cast<u64>(key_of(b)) << 32 : 0ull;
     } else {
-        bound = block_bound(mx > -INFINITY ? key_of(mx) : 0u, p.n_out, slots);
+        bound = block_bound(mx > -INFINITY ? key_of(mx) : 0u, p.n_out, reinterpret_cast<uint32_t(*)[32]>(pool.key), sets);
     }
 
     float sum = 0.f;
     if (top > -INFINITY) {
         const float shift = top * LOG2E;
+        float2 part = make_float2(0.f, 0.f);
 #pragma unroll 4
         for (int i = 0; i < NV; ++i) {
-            float x[V], part = 0.f;
+            float x[V];
             elements<T>(mine[i * BS_THREADS], x);
 #pragma unroll
-            for (int k = 0; k < V; ++k) part += ex2(fmaf(x[k], LOG2E, -shift));
-            sum += part;
+            for (int k = 0; k < V; k += 2) {
+                const float2 y = fma2(make_float2(x[k], x[k + 1]), make_float2(LOG2E, LOG2E), make_float2(-shift, -shift));
+                part = add2(part, make_float2(ex2(y.x), ex2(y.y)));
+            }
         }
+        sum = part.x + part.y;
         if (sum != sum) {  // NaN among the logits: once more without them
             sum = 0.f;
 #pragma unroll 1
@@ -340,7 +361,7 @@ __global__ void __launch_bounds__(BS_THREADS) beam_tile_kernel(const __grid_cons
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     if (lane == 0) wl[warp] = sum;
-    const int n = collect(pool, bound, p.n_out, [&](u64 bk, uint32_t bi) {
+    const int n = collect(pool, bound, p.n_out, [&](u64 bk, uint32_t) {
         const float floor_v = bk >> 32 ? value_of(static_cast<uint32_t>(bk >> 32)) : -INFINITY;
         // which vectors hold a candidate, then only those, element by element
         unsigned hits = 0;
@@ -355,8 +376,8 @@ __global__ void __launch_bounds__(BS_THREADS) beam_tile_kernel(const __grid_cons
             for (int k = 0; k < V; ++k)
                 if (x[k] >= floor_v && x[k] > -INFINITY) {
                     const uint32_t e = static_cast<uint32_t>(first + i * BS_THREADS) * V - skew + k;
-                    const u64 key = static_cast<u64>(key_of(x[k])) << 32;
-                    if (!before(bk, bi, key, e)) pool_add(pool, key, e);
+                    const u64 key = static_cast<u64>(key_of(x[k])) << 32 | static_cast<uint32_t>(~e);
+                    if (key >= bk) pool.add(key, 0);
                 }
         }
     });
@@ -367,15 +388,18 @@ __global__ void __launch_bounds__(BS_THREADS) beam_tile_kernel(const __grid_cons
         p.tile_ml[blockIdx.x] = make_float2(m, l);
     }
     u64* out = p.tile_top + static_cast<long long>(blockIdx.x) * p.n_out;
-    for (int i = tid; i < p.n_out; i += BS_THREADS) out[i] = i < n ? pool.key[i] | static_cast<uint32_t>(~pool.idx[i]) : 0ull;
+    for (int i = tid; i < p.n_out; i += BS_THREADS) out[i] = i < n ? pool.key[i] : 0ull;
 }
 
 // One CTA per group: log-sums of its beams, then the order of what the tiles kept.
 __global__ void __launch_bounds__(BS_THREADS) beam_join_kernel(const __grid_constant__ SelectParams p) {
-    __shared__ Pool pool;
-    __shared__ uint32_t slots[BS_WARPS];
+    using Candidates = Pool<BS_CAP, false>;
+    __shared__ Candidates pool;
+    __shared__ uint32_t sets[4];
     __shared__ double offset[BS_MAX_BEAMS];  // score - lse
     __shared__ uint8_t state[BS_MAX_BEAMS];  // 0: nothing, 1: its row, 2: finished
+    __shared__ int open[BS_CAP];
+    __shared__ unsigned n_open;
     izb::pdl_launch_dependents();
     izb::pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -429,12 +453,27 @@ __global__ void __launch_bounds__(BS_THREADS) beam_join_kernel(const __grid_cons
         uint32_t idx;
         if (list_at(l, 0, key, idx)) mine = max(mine, static_cast<uint32_t>(key >> 32));
     }
-    const u64 bound = block_bound(mine, p.n_out, slots);
+    const u64 bound = block_bound(mine, p.n_out, reinterpret_cast<uint32_t(*)[32]>(pool.key), sets);
+    // the lists whose first pair is not behind the bound, BS_CAP at a time, then their pairs, all of them at once (one after
+    // the other, list by list, every pair was a trip to memory: 190 us for 64 of 8 x 10 lists)
     const int n = collect(pool, bound, p.n_out, [&](u64 bk, uint32_t bi) {
-        for (int l = tid; l < lists; l += BS_THREADS) {
-            u64 key;
-            uint32_t idx;
-            for (int i = 0; list_at(l, i, key, idx) && !before(bk, bi, key, idx); ++i) pool_add(pool, key, idx);
+        for (int l0 = 0; l0 < lists; l0 += BS_CAP) {
+            if (tid == 0) n_open = 0;
+            __syncthreads();
+            for (int l = l0 + tid; l < min(lists, l0 + BS_CAP); l += BS_THREADS) {
+                u64 key;
+                uint32_t idx;
+                if (list_at(l, 0, key, idx) && !Candidates::before(bk, bi, key, idx)) open[atomicAdd(&n_open, 1u)] = l;
+            }
+            __syncthreads();
+            const int pairs = static_cast<int>(n_open) * p.n_out;
+            for (int e = tid; e < pairs; e += BS_THREADS) {
+                u64 key;
+                uint32_t idx;
+                const int l = e / p.n_out;
+                if (list_at(open[l], e - l * p.n_out, key, idx) && !Candidates::before(bk, bi, key, idx)) pool.add(key, idx);
+            }
+            __syncthreads();
         }
     });
     for (int i = tid; i < p.n_out; i += BS_THREADS) {
