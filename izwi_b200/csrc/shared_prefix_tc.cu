@@ -328,6 +328,21 @@ __device__ __forceinline__ void convert_role(const Params& p, int kv, int warp, 
     if (!ok) sh.failed = 1;
 }
 
+// The sequence of its group and the query head (of those of the KV head) a row of the block stands for, and a step of rows.
+struct HeadStep {
+    int s, h;
+    __device__ __forceinline__ HeadStep(const Params& p, int rows) : s(rows / p.g), h(rows - s * p.g) {}
+};
+struct HeadRow {
+    int s, h;
+    __device__ __forceinline__ HeadRow(const Params& p, int row) : s(row / p.g), h(row - s * p.g) {}
+    __device__ __forceinline__ void advance(const HeadStep& by, const Params& p) {
+        s += by.s;
+        h += by.h;
+        if (h >= p.g) { h -= p.g; ++s; }
+    }
+};
+
 template <int D, int Q, int CONV>
 __global__ void __launch_bounds__(Roles<Q, CONV>::THREADS, 1)
     shared_prefix_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Maps maps, int wide) {
@@ -470,17 +485,19 @@ __global__ void __launch_bounds__(Roles<Q, CONV>::THREADS, 1)
         // the query rows, K-major, all of a thread's 16-byte pieces under way at once
         {
             constexpr int C = D / 8, STEP = 256 / C, B = CODES ? 8 : 16;
-            const int c = tid % C;
-            for (int r0 = tid / C; r0 < block_rows; r0 += B * STEP) {
+            const int c = tid % C, start = tid / C;
+            HeadRow at(p, row0 + start), again = at;
+            const HeadStep by(p, STEP);
+            for (int r0 = start; r0 < block_rows; r0 += B * STEP) {
                 uint4 x[B];
 #pragma unroll
                 for (int j = 0; j < B; ++j) {
-                    const int r = r0 + j * STEP, nth = !wide && r >= twin ? r - twin : r, at = row0 + nth;
+                    const int r = r0 + j * STEP;
+                    if (!wide && r == twin + start) at = again;
                     x[j] = make_uint4(0u, 0u, 0u, 0u);
-                    if (nth < n_rows) {
-                        const int s = at / p.g, h = at - s * p.g;
-                        x[j] = *reinterpret_cast<const uint4*>(p.q + (seq0 + s) * p.ld_q + static_cast<long long>(kh * p.g + h) * D + c * 8);
-                    }
+                    if ((!wide && r >= twin ? r - twin : r) < n_rows)
+                        x[j] = *reinterpret_cast<const uint4*>(p.q + (seq0 + at.s) * p.ld_q + static_cast<long long>(kh * p.g + at.h) * D + c * 8);
+                    at.advance(by, p);
                 }
 #pragma unroll
                 for (int j = 0; j < B; ++j) {
@@ -615,9 +632,13 @@ __global__ void __launch_bounds__(Roles<Q, CONV>::THREADS, 1)
         named_bar_sync(3, 256);
         const int chunks = p.prefix.n_chunks + p.own.n_chunks;
         constexpr int LANES = D / 4, RW = 32 / LANES;  // lanes of a row, rows of a warp at a time
+        HeadRow at(p, row0 + warp * RW + lane / LANES);
+        const HeadStep by(p, 8 * RW);
+#pragma unroll 4
         for (int r = warp * RW + lane / LANES; r < n_rows; r += 8 * RW) {
-            const int d = (lane % LANES) * 4, at = row0 + r, s = at / p.g, h = at - s * p.g;
-            const long long slot = (static_cast<long long>(seq0 + s) * p.heads + kh * p.g + h) * chunks + chunk;
+            const int d = (lane % LANES) * 4;
+            const long long slot = (static_cast<long long>(seq0 + at.s) * p.heads + kh * p.g + at.h) * chunks + chunk;
+            at.advance(by, p);
             float4 x = *reinterpret_cast<const float4*>(stage + r * LD + d);  // row r & 127 of set r >> 7
             float2 a = sh.ml[r >> 7][r & 127];
             if (!wide && n_tiles > 1) {
