@@ -14,7 +14,8 @@ namespace {
 // Inside a row the order is that of the logits, so one pass over them yields, for every tile of a row, the tile's
 // maximum, its sum of exp(x - maximum) and its n_out largest (value, index) pairs; a second launch forms lse_b from
 // the tiles, the totals of the few pairs that are left (in fp64: candidates of different beams are ranked by them),
-// and their order.  Bound by reading the logits once.
+// and their order.  32 x 8 rows of 151,936 bf16 logits: 29.6 us with the join (floor 11.9: reading them once), bound by issue
+// slots; some 40 instructions for eight logits and 300 a thread for a tile's ends.
 
 constexpr int BS_THREADS = 256;
 constexpr int BS_WARPS = BS_THREADS / 32;
@@ -526,7 +527,8 @@ cudaError_t launch_tiles(izb_ctx* ctx, cudaStream_t s, const SelectParams& p, in
 // copied.  Its last, partly filled page will be written by every child, so each child needs one of its own: the
 // first child of a parent keeps the parent's page, and the others take the pages of beams without a child, in
 // ascending order (there are exactly as many), and copy the rows held so far.  A page that is read is kept by
-// somebody and a page that is written belonged to nobody any more, so copies of one call never meet.
+// somebody and a page that is written belonged to nobody any more, so copies of one call never meet.  Bound by DRAM:
+// 16 x 8 beams, 36 layers of bf16 pages 111.7 us = 5.6 TB/s of reads and writes; 4 beams, 4 layers 3.0 us, one launch.
 
 constexpr int RO_MAX_BEAMS = 32;
 constexpr int RO_MAX_LAYERS = 64;
@@ -632,7 +634,8 @@ __global__ void __launch_bounds__(RO_THREADS) kv_pages_reorder_kernel(const __gr
 // beams, `beams` lanes hold a step's parents, so a step of the walk is a shuffle among them; and the steps are cut into
 // chunks, 32 / beams of them side by side in a warp, one warp after the other: first every chunk maps all beams at its
 // end to beams at its start and a warp's chunks are chained into one map, then the warps' maps are chained, and then
-// every chunk is walked again from where the walks enter it, writing tokens.
+// every chunk is walked again from where the walks enter it, writing tokens.  Bound by that chain: 32 x 8 walks of 4,096
+// steps 15.7 us (a group's warps in four CTAs of a cluster; 26.6 in one), 5 of 37 steps 3.5 us, one launch.
 constexpr int TR_WARPS = 32;
 constexpr int TR_AHEAD = 16;    // steps whose rows a lane has in flight
 constexpr int TR_NONE = 0xFF;   // a walk that has left [0, beams)

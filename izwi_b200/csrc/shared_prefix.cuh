@@ -83,8 +83,8 @@ struct CodeBits {
         return hfma2(low, 0x3F803F80u, Q == IZB_KV_INT8 ? lop3<0xAE>(x, top, bias) : bias);  // (~x & top) | bias
     }
 };
-// code * scale rounded to bf16 as the stored value is defined.  The fp32 scale enters as two bf16 parts; the product
-// with the small part is rounded to 8 bits at 2^-8 of the value, so the sum's one rounding sees the product to 2^-17.
+// code * scale rounded to bf16 as the stored value is defined.  The fp32 scale enters as two bf16 parts; the small
+// part, 2^-8 of it at most, and its product are rounded to 8 bits each, so the sum's one rounding sees the product to 2^-15.
 __device__ __forceinline__ uint32_t q4_value(uint32_t code2, uint32_t hi2, uint32_t lo2) { return hfma2(code2, hi2, hmul2(code2, lo2)); }
 // the two parts of two scales side by side
 __device__ __forceinline__ void split_scales(float a, float b, uint32_t& hi2, uint32_t& lo2) {

@@ -5,9 +5,10 @@ Tolerance.  The kernel's result differs from the exact one by the rounding of th
 bf16 step), the rounding of the weights for the product with v (2^-8 of each term, so 2^-8 of A = sum p |v| / sum p), and
 fp32 arithmetic: scores of D products (D 2^-24 of B = scale sum |q| |k|, which moves a weight by that much, both in the
 numerator and in the sum) and accumulation over the tokens (T 2^-24 of A).  Q4_0 scales that are no bf16 numbers: a
-stored value is the product of code and scale rounded to bf16; the kernel may land on the neighbour when the product is
-within 2^-17 of a tie, so it is held to the unrounded product, from which both lie at most 2^-8 (1 + 2^-8) away: weights
-move by that times 2 B, values by that."""
+stored value is the product of code and scale rounded to bf16; the kernel splits the scale into two bf16 parts (the second
+at most 2^-8 of it and rounded by 2^-8 of itself, its product with the code once more: 2^-15 in all) and may land on the
+neighbour when the product is that near a tie, so it is held to the unrounded product, from which it lies at most
+2^-8 + 2^-15 (1 + 2^-8) away: weights move by that times 2 B, values by that."""
 import math
 
 import numpy as np
@@ -136,7 +137,7 @@ def test_q4_0_scales_of_full_precision(cuda, d):
     rng = np.random.default_rng(8)
     prefix = Pool(rng, cuda, [150], 2, d, 64, "q4_0", bf16_scales=False)
     suffix = Pool(rng, cuda, [9, 70], 2, d, 64, "q4_0", bf16_scales=False)
-    check(rng, cuda, 2, 4, prefix, suffix, value_off=HALF * (1 + HALF))
+    check(rng, cuda, 2, 4, prefix, suffix, value_off=HALF + 2 ** -15 * (1 + HALF))
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.05, 0.5])
@@ -344,3 +345,18 @@ def test_rows_of_any_stride_and_address(cuda, quant, seqs, heads, slens):
         o.seq_lens.data_ptr(), room.data_ptr() + 2, 1, seqs, heads, p.max_tokens, o.max_tokens, heads * 128, ld, 128 ** -0.5, ws.data_ptr(), need), "call")
     got = room[1:].reshape(seqs, ld)
     assert torch.equal(got[:, :-3], want) and (got[:, -3:] == 7).all() and room[0] == 7
+
+
+@pytest.mark.parametrize("quant", ["none", "int8", "q4_0"])
+def test_many_rows_without_prefix_or_without_own_tokens(cuda, quant):
+    """Bounds of zero leave a cache out, whatever its lengths say; with both at zero every row is zero."""
+    from izwi_b200 import ops, paged
+    rng = np.random.default_rng(41)
+    prefix, own = Pool(rng, cuda, [70, 3], 2, 64, 16, quant), Pool(rng, cuda, [1, 0, 130, 17] * 10, 2, 64, 16, quant)
+    none = Pool(rng, cuda, [0, 0], 2, 64, 16, quant)
+    none.cache = prefix.cache
+    check(rng, cuda, 20, 8, none, own, max_prefix_len=0)
+    q = torch.from_numpy(rng.normal(0, 1, (40, 8, 64)).astype(np.float32)).to(cuda).to(torch.bfloat16)
+    assert torch.equal(paged.shared_prefix_attention(q, prefix.cache, own.cache, max_seq_len=0), paged.shared_prefix_attention(q, prefix.cache, None))
+    assert (paged.shared_prefix_attention(q, prefix.cache, own.cache, max_prefix_len=0, max_seq_len=0) == 0).all()
+    ops.Context.get(0).check()
