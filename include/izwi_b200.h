@@ -570,7 +570,7 @@ int32_t izb_beam_select(izb_ctx* ctx, izb_stream stream, const void* logits, int
  * further children get the pages of beams that have no child, into which the rows held so far (and their
  * scales) are copied; later entries stay.  parents [groups * beams] int32, each in [0, beams).  A group with a parent
  * outside that range, unequal lengths or a length beyond its table keeps its rows unchanged and makes the
- * next izb_ctx_check return IZB_ERR_BAD_ARG.  beams <= 32. */
+ * next izb_ctx_check return IZB_ERR_BAD_ARG.  beams <= 32, groups * beams <= 65535. */
 int32_t izb_kv_pages_reorder(izb_ctx* ctx, izb_stream stream, const izb_kv_pages* layers, int32_t n_layers,
                              const int32_t* parents, int64_t groups, int32_t beams, const int32_t* seq_lens,
                              int32_t* page_table_out);

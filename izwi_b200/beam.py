@@ -60,7 +60,7 @@ class BeamSearch:
 
 
 class Qwen3BeamDecoder:
-    """Beam search over a Qwen3 decoder from prompts whose keys and values are in dense caches.  The prompt of each sequence
+    """Beam search over a Qwen3 decoder from prompts of one length whose keys and values are in dense caches.  The prompt of each sequence
     is stored once per layer in pages (`quantization`); the beams add tokens to pages of their own (`own_quantization`)."""
 
     def __init__(self, decoder: Qwen3Decoder, caches: list[KvCache], prompt_len: int, beams: int, max_new_tokens: int, eos: int = -1,
@@ -83,6 +83,8 @@ class Qwen3BeamDecoder:
 
     def forward(self, tokens: torch.Tensor) -> torch.Tensor:
         """One token of every beam, [groups * beams] int32, through the layers: logits [groups * beams, vocab] fp32."""
+        if self.held >= self.search.max_steps:
+            raise ValueError(f"forward: the beams hold {self.held} tokens, all they were given room for")
         dec, w = self.decoder, self.decoder.w
         b, pos = tokens.numel(), self.prompt_len + self.held
         cos_half, sin_half = dec.rope_tables(pos, b)

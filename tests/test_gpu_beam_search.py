@@ -160,6 +160,9 @@ def test_decoder_follows_the_search(cuda, quant):
     ops.Context.get(0).check()
     sequences, scores = run.search.sequences(2)
     assert sequences.shape == (groups, 2, new) and torch.isfinite(scores).all()
+    run.forward(tokens)
+    with pytest.raises(ValueError):        # no room for more
+        run.forward(tokens)
     # the whole loop in one call gives the same
     again = beam.Qwen3BeamDecoder(dec, caches, prompt, beams, new, eos, quantization=quant, page_size=4)
     whole, value = again.generate(logits, n_best=2)
