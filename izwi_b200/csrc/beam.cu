@@ -635,24 +635,27 @@ __global__ void __launch_bounds__(RO_THREADS) kv_pages_reorder_kernel(const __gr
 // chunks, 32 / beams of them side by side in a warp, one warp after the other: first every chunk maps all beams at its
 // end to beams at its start and a warp's chunks are chained into one map, then the warps' maps are chained, and then
 // every chunk is walked again from where the walks enter it, writing tokens.  Bound by that chain: 32 x 8 walks of 4,096
-// steps 15.7 us (a group's warps in four CTAs of a cluster; 26.6 in one), 5 of 37 steps 3.5 us, one launch.
+// steps 13.1 us, 14.1 with nothing in L2 (a group's warps in four CTAs of a cluster, 32 steps a lane in flight; 15.7 and 21.5
+// with 16; one CTA 26.6), 5 of 37 steps 3.5 us, one launch.
 constexpr int TR_WARPS = 32;
-constexpr int TR_AHEAD = 16;    // steps whose rows a lane has in flight
 constexpr int TR_NONE = 0xFF;   // a walk that has left [0, beams)
 
-// Rows s0 .. s0 + 15 of a lane's column (those below n), `ld` apart; s0 + 16 <= n for every lane of the warp: no tests.
-__device__ __forceinline__ void trace_rows(int (&r)[TR_AHEAD], const int* from, long long ld, int s0, int n, bool whole) {
+// Rows s0 .. s0 + AHEAD - 1 of a lane's column (those below n), `ld` apart; whole: none is past n for any lane of the warp.
+template <int AHEAD>
+__device__ __forceinline__ void trace_rows(int (&r)[AHEAD], const int* from, long long ld, int s0, int n, bool whole) {
     const int* at = from + s0 * ld;
     if (whole) {
 #pragma unroll
-        for (int j = 0; j < TR_AHEAD; ++j, at += ld) r[j] = __ldg(at);
+        for (int j = 0; j < AHEAD; ++j, at += ld) r[j] = __ldg(at);
     } else {
 #pragma unroll
-        for (int j = 0; j < TR_AHEAD; ++j, at += ld) r[j] = s0 + j < n ? __ldg(at) : 0;
+        for (int j = 0; j < AHEAD; ++j, at += ld) r[j] = s0 + j < n ? __ldg(at) : 0;
     }
 }
 
-__global__ void __launch_bounds__(TR_WARPS * 32)
+// AHEAD: steps whose rows a lane has in flight; more than 16 only where a CTA has a quarter of the warps.
+template <int AHEAD>
+__global__ void __launch_bounds__(AHEAD > 16 ? TR_WARPS * 8 : TR_WARPS * 32)
     beam_trace_chunks_kernel(const int* __restrict__ parents, const int* __restrict__ tokens, const int* __restrict__ last,
                              int* __restrict__ out, int steps, int beams, int picks, long long groups, long long ld_out, int chunk,
                              int ranks, int* status) {
@@ -686,20 +689,20 @@ __global__ void __launch_bounds__(TR_WARPS * 32)
     auto back = [&](int at, int to) { return at == TR_NONE || static_cast<unsigned>(to) >= static_cast<unsigned>(beams) ? TR_NONE : to; };
 
     // steps that fit one read are read once, tokens and the walks' ends with them: a short trace waits for memory once
-    const bool once = most <= TR_AHEAD;
-    int r[TR_AHEAD], t[TR_AHEAD];
+    const bool once = most <= AHEAD;
+    int r[AHEAD], t[AHEAD];
     if (once) {
-        trace_rows(r, par, ld, 0, n, even && n == TR_AHEAD);
-        trace_rows(t, tok, ld, 0, n, even && n == TR_AHEAD);
+        trace_rows(r, par, ld, 0, n, even && n == AHEAD);
+        trace_rows(t, tok, ld, 0, n, even && n == AHEAD);
     }
     int end = warp == 0 && lane < beams && lane < picks ? last[group * picks + lane] : -1;
 
     int mine = me;  // beam `me` at the end of this lane's chunk -> beam at its start
     if (chunks > 1 && (side > 1 || warp > 0)) {  // nothing leads on from the first chunk of all
-        for (int s0 = (most - 1) / TR_AHEAD * TR_AHEAD; s0 >= 0; s0 -= TR_AHEAD) {
-            if (!once) trace_rows(r, par, ld, s0, n, even && n && s0 + TR_AHEAD <= most);
+        for (int s0 = (most - 1) / AHEAD * AHEAD; s0 >= 0; s0 -= AHEAD) {
+            if (!once) trace_rows(r, par, ld, s0, n, even && n && s0 + AHEAD <= most);
 #pragma unroll
-            for (int j = TR_AHEAD - 1; j >= 0; --j) {
+            for (int j = AHEAD - 1; j >= 0; --j) {
                 const int to = __shfl_sync(0xFFFFFFFFu, r[j], (base + mine) & 31);
                 if (s0 + j < n) mine = back(mine, to);
             }
@@ -737,12 +740,12 @@ __global__ void __launch_bounds__(TR_WARPS * 32)
             if (k > sub && at != TR_NONE) at = to;
         }
         bool lost = false;
-        for (int s0 = (most - 1) / TR_AHEAD * TR_AHEAD; s0 >= 0; s0 -= TR_AHEAD) {
-            const bool whole = even && n && s0 + TR_AHEAD <= most;
+        for (int s0 = (most - 1) / AHEAD * AHEAD; s0 >= 0; s0 -= AHEAD) {
+            const bool whole = even && n && s0 + AHEAD <= most;
             if (!once) trace_rows(r, par, ld, s0, n, whole);
             if (!once || p0 > 0) trace_rows(t, tok, ld, s0, n, whole);  // the tokens' registers become the results
 #pragma unroll
-            for (int j = TR_AHEAD - 1; j >= 0; --j) {
+            for (int j = AHEAD - 1; j >= 0; --j) {
                 const int from = (base + at) & 31;
                 const int token = __shfl_sync(0xFFFFFFFFu, t[j], from), to = __shfl_sync(0xFFFFFFFFu, r[j], from);
                 t[j] = at == TR_NONE ? -1 : token;
@@ -751,12 +754,12 @@ __global__ void __launch_bounds__(TR_WARPS * 32)
                     at = back(at, to);
                 }
             }
-            if (walks && wide && s0 + TR_AHEAD <= n) {
+            if (walks && wide && s0 + AHEAD <= n) {
 #pragma unroll
-                for (int j = 0; j < TR_AHEAD; j += 4) *reinterpret_cast<int4*>(dst + s0 + j) = make_int4(t[j], t[j + 1], t[j + 2], t[j + 3]);
+                for (int j = 0; j < AHEAD; j += 4) *reinterpret_cast<int4*>(dst + s0 + j) = make_int4(t[j], t[j + 1], t[j + 2], t[j + 3]);
             } else if (walks) {
 #pragma unroll
-                for (int j = 0; j < TR_AHEAD; ++j)
+                for (int j = 0; j < AHEAD; ++j)
                     if (s0 + j < n) dst[s0 + j] = t[j];
             }
         }
@@ -914,10 +917,12 @@ int32_t izb_beam_trace(izb_ctx* ctx, izb_stream stream, const int32_t* parents, 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (beams <= 32) {
         // one chunk for every place of the CTA's warps, of whole reads ahead
-        const int64_t places = TR_WARPS * (32 / beams), chunk = ((steps + places - 1) / places + TR_AHEAD - 1) / TR_AHEAD * TR_AHEAD;
+        const int64_t places = TR_WARPS * (32 / beams), chunk = ((steps + places - 1) / places + 15) / 16 * 16;
         const int64_t warps = ((steps + chunk - 1) / chunk + 32 / beams - 1) / (32 / beams);  // a short trace is one warp's
         const int ranks = warps >= 8 && groups <= ctx->sm_count ? 4 : 1;
-        IZB_CUDA_TRY(izb::launch_chained_cluster(ctx, ranks, beam_trace_chunks_kernel, dim3(static_cast<unsigned>(groups * ranks)),
+        // a lane's chunk of up to 32 steps is read once where the registers allow it
+        auto kern = ranks == 4 && chunk > 16 ? beam_trace_chunks_kernel<32> : beam_trace_chunks_kernel<16>;
+        IZB_CUDA_TRY(izb::launch_chained_cluster(ctx, ranks, kern, dim3(static_cast<unsigned>(groups * ranks)),
                                                  dim3(static_cast<unsigned>((warps + ranks - 1) / ranks * 32)), 0, st, parents, tokens, last, out, static_cast<int>(steps), beams, picks,
                                                  static_cast<long long>(groups), static_cast<long long>(ld_out), static_cast<int>(chunk), ranks,
                                                  ctx->d_status + 6));
