@@ -528,11 +528,12 @@ cudaError_t launch_tiles(izb_ctx* ctx, cudaStream_t s, const SelectParams& p, in
 // first child of a parent keeps the parent's page, and the others take the pages of beams without a child, in
 // ascending order (there are exactly as many), and copy the rows held so far.  A page that is read is kept by
 // somebody and a page that is written belonged to nobody any more, so copies of one call never meet.  Bound by DRAM:
-// 16 x 8 beams, 36 layers of bf16 pages 111.7 us = 5.6 TB/s of reads and writes; 4 beams, 4 layers 3.0 us, one launch.
+// 16 x 8 beams, 36 layers of bf16 pages 98.2 us = 6.4 TB/s of reads and writes; 4 beams, 4 layers 3.0 us, one launch.
 
 constexpr int RO_MAX_BEAMS = 32;
 constexpr int RO_MAX_LAYERS = 64;
 constexpr int RO_THREADS = 256;
+constexpr int RO_WAVES = 8;  // of five CTAs an SM
 
 struct LayerPtrs {
     uint8_t* k;
@@ -553,11 +554,20 @@ struct ReorderParams {
     int beams, page_size, n_layers, splits;
 };
 
-// grid (layers * 2 * splits, groups * beams): CTA (0, child) also writes the child's table row
+// grid (CTAs of a child, groups * beams): CTA (0, child) also writes the child's table row
 __global__ void __launch_bounds__(RO_THREADS) kv_pages_reorder_kernel(const __grid_constant__ ReorderParams p) {
     izb::pdl_launch_dependents();
     izb::pdl_wait();
     __shared__ int sh_parent, sh_src, sh_dst, sh_full, sh_held;
+    // units of 32 KB of a page of K or V of a layer, in turn among the CTAs of the child
+    int unit = blockIdx.x, split, which, layer;
+    auto where = [&]() {
+        const int page = unit / p.splits;
+        split = unit - page * p.splits;
+        which = page & 1;
+        layer = page >> 1;
+    };
+    where();
     const int child = blockIdx.y % p.beams, row0 = blockIdx.y - child;
     if (threadIdx.x < 32) {
         const int lane = threadIdx.x;
@@ -604,14 +614,14 @@ __global__ void __launch_bounds__(RO_THREADS) kv_pages_reorder_kernel(const __gr
             out[c] = c < full ? theirs[c] : (c == full && held) ? sh_dst : mine[c];
     }
     if (!held || sh_src == sh_dst) return;
-    const int split = blockIdx.x % p.splits, which = (blockIdx.x / p.splits) & 1, layer = blockIdx.x / (2 * p.splits);
-    uint8_t* values = which ? p.layer[layer].v : p.layer[layer].k;
-    float* scales = which ? p.layer[layer].v_scales : p.layer[layer].k_scales;
-    const uint4* src = reinterpret_cast<const uint4*>(values + sh_src * p.page_bytes);
-    uint4* dst = reinterpret_cast<uint4*>(values + sh_dst * p.page_bytes);
     const int n = static_cast<int>(held * p.row_bytes / 16);
     constexpr int UN = 8;
-    for (int i0 = split * RO_THREADS * UN + threadIdx.x; i0 < n; i0 += p.splits * RO_THREADS * UN) {
+    for (; unit < p.n_layers * 2 * p.splits; unit += gridDim.x, where()) {
+        uint8_t* values = which ? p.layer[layer].v : p.layer[layer].k;
+        float* scales = which ? p.layer[layer].v_scales : p.layer[layer].k_scales;
+        const uint4* src = reinterpret_cast<const uint4*>(values + sh_src * p.page_bytes);
+        uint4* dst = reinterpret_cast<uint4*>(values + sh_dst * p.page_bytes);
+        const int i0 = split * RO_THREADS * UN + threadIdx.x;
         uint4 w[UN];
 #pragma unroll
         for (int j = 0; j < UN; ++j)
@@ -619,11 +629,20 @@ __global__ void __launch_bounds__(RO_THREADS) kv_pages_reorder_kernel(const __gr
 #pragma unroll
         for (int j = 0; j < UN; ++j)
             if (i0 + j * RO_THREADS < n) __stcs(dst + i0 + j * RO_THREADS, w[j]);
-    }
-    if (scales && split == 0) {
-        const int m = p.row_scales ? held * p.row_scales : p.page_scales;
-        for (int i = threadIdx.x; i < m; i += RO_THREADS)
-            scales[static_cast<long long>(sh_dst) * p.page_scales + i] = scales[static_cast<long long>(sh_src) * p.page_scales + i];
+        if (scales && split == 0) {
+            const int m = p.row_scales ? held * p.row_scales : p.page_scales;
+            const float* from = scales + static_cast<long long>(sh_src) * p.page_scales;
+            float* to = scales + static_cast<long long>(sh_dst) * p.page_scales;
+            for (int i = threadIdx.x; i < m; i += RO_THREADS * UN) {
+                float x[UN];
+#pragma unroll
+                for (int j = 0; j < UN; ++j)
+                    if (i + j * RO_THREADS < m) x[j] = from[i + j * RO_THREADS];
+#pragma unroll
+                for (int j = 0; j < UN; ++j)
+                    if (i + j * RO_THREADS < m) to[i + j * RO_THREADS] = x[j];
+            }
+        }
     }
 }
 
@@ -893,13 +912,16 @@ int32_t izb_kv_pages_reorder(izb_ctx* ctx, izb_stream stream, const izb_kv_pages
     p.beams = beams;
     p.page_size = a.page_size;
     p.n_layers = n_layers;
-    // 32 KB of a page per CTA and trip
-    const long long per = RO_THREADS * 8 * 16;
-    long long splits = (p.page_bytes + per - 1) / per;
-    p.splits = static_cast<int>(splits > 64 ? 64 : splits);
+    // 32 KB of a page per CTA and trip; a CTA finds out first what there is to copy, so a big batch gets no more of them than
+    // keep the SMs busy eight times over (16 x 8 beams, 36 layers: bf16 98.2 us against 111.6 with a CTA for every 32 KB, Int8
+    // 45.9 against 53.3, Q4_0 39.0 against 48.3; one group 10.8 against 10.0)
+    p.splits = static_cast<int>((p.page_bytes + RO_THREADS * 128 - 1) / (RO_THREADS * 128));
+    const int64_t units = static_cast<int64_t>(n_layers) * 2 * p.splits;
+    const int64_t most = (static_cast<int64_t>(RO_WAVES) * 5 * ctx->sm_count + groups * beams - 1) / (groups * beams);
+    const unsigned per_child = static_cast<unsigned>(units < most ? units : most);
     izb::DeviceGuard guard(ctx->device);
     if (!guard.ok) return IZB_ERR_LAUNCH;
-    IZB_CUDA_TRY(izb::launch_chained(ctx, kv_pages_reorder_kernel, dim3(static_cast<unsigned>(n_layers * 2 * p.splits), static_cast<unsigned>(groups * beams)),
+    IZB_CUDA_TRY(izb::launch_chained(ctx, kv_pages_reorder_kernel, dim3(per_child, static_cast<unsigned>(groups * beams)),
                                      dim3(RO_THREADS), 0, static_cast<cudaStream_t>(stream), p));
     ctx->launches.fetch_add(1, std::memory_order_relaxed);
     return IZB_OK;
