@@ -665,31 +665,47 @@ __global__ void __launch_bounds__(128)
     shared_prefix_join_kernel(const __grid_constant__ Params p, __nv_bfloat16* __restrict__ out, long long ld_out) {
     izb::pdl_launch_dependents();
     izb::pdl_wait();
-    constexpr int E = D / 32;
+    constexpr int E = D / 32, AHEAD = 4;
     __shared__ float sm_acc[4][D], sm_m[4], sm_l[4];
     const int row = blockIdx.x, seq = row / p.heads, head = row - seq * p.heads;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int chunks = p.prefix.n_chunks + p.own.n_chunks;
-    const int np = prefix_chunks_of(p, seq / p.seqs);
-    const int no = p.own.n_chunks ? (length_of(p.own, seq) + p.own.chunk - 1) / p.own.chunk : 0;
+    const int len_p = p.prefix.n_chunks ? length_of(p.prefix, seq / p.seqs) : 0, len_o = p.own.n_chunks ? length_of(p.own, seq) : 0;
     const long long base = static_cast<long long>(row) * chunks;
+    auto used = [&](int c) { return c < p.prefix.n_chunks ? c * p.prefix.chunk < len_p : c < chunks && (c - p.prefix.n_chunks) * p.own.chunk < len_o; };
     float m = -INFINITY, l = 0.f, a[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) a[e] = 0.f;
-#pragma unroll 4
-    for (int c = warp; c < np + no; c += 4) {
-        const long long slot = base + (c < np ? c : p.prefix.n_chunks + c - np);
-        const float2 x = p.ml[slot];
-        float v[E];
+    for (int c0 = warp; c0 < chunks; c0 += 4 * AHEAD) {
+        // The first results are read while the lengths are on their way: their places exist, and what is not in use is not used.
+        float2 x[AHEAD];
+        float v[AHEAD][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = p.acc[slot * D + lane * E + e];
-        const float n = fmaxf(m, x.x);
-        const float u = n == -INFINITY ? 0.f : n;
-        const float f = ex2(m - u), g = ex2(x.x - u);
-        l = l * f + x.y * g;
-        m = n;
+        for (int i = 0; i < AHEAD; ++i) {
+            const int c = c0 + 4 * i;
+            if (c0 == warp ? c < chunks : used(c)) {
+                x[i] = p.ml[base + c];
+                const float* from = p.acc + (base + c) * D + lane * E;
+                if constexpr (E == 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(from);
+                    v[i][0] = y.x; v[i][1] = y.y; v[i][2] = y.z; v[i][3] = y.w;
+                } else {
+                    const float2 y = *reinterpret_cast<const float2*>(from);
+                    v[i][0] = y.x; v[i][1] = y.y;
+                }
+            }
+        }
 #pragma unroll
-        for (int e = 0; e < E; ++e) a[e] = a[e] * f + v[e] * g;
+        for (int i = 0; i < AHEAD; ++i) {
+            if (!used(c0 + 4 * i)) continue;
+            const float n = fmaxf(m, x[i].x);
+            const float u = n == -INFINITY ? 0.f : n;
+            const float f = ex2(m - u), g = ex2(x[i].x - u);
+            l = l * f + x[i].y * g;
+            m = n;
+#pragma unroll
+            for (int e = 0; e < E; ++e) a[e] = a[e] * f + v[i][e] * g;
+        }
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) sm_acc[warp][lane * E + e] = a[e];
