@@ -406,18 +406,24 @@ __global__ void __launch_bounds__(BS_THREADS) beam_join_kernel(const __grid_cons
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int group = blockIdx.x, row0 = group * p.beams;
     if (tid == 0) pool.count = 0;
+    // What the tiles left is read while the scores are on their way: the places exist, and those of rows that do not count
+    // are not used.
+    const int lists = p.beams * p.tiles;
+    const u64* lists_from = p.tile_top + static_cast<long long>(row0) * p.tiles * p.n_out;
+    const u64 first = tid < lists ? lists_from[static_cast<long long>(tid) * p.n_out] : 0ull;
     for (int b = warp; b < p.beams; b += BS_WARPS) {
+        const float2* ml = p.tile_ml + static_cast<long long>(row0 + b) * p.tiles;
+        float2 x0 = lane < p.tiles ? ml[lane] : make_float2(-INFINITY, 0.f);
         const float score = p.scores[row0 + b];
         const bool alive = isfinite(score), done = p.finished && p.finished[row0 + b];
         if (alive && !done) {
-            const float2* ml = p.tile_ml + static_cast<long long>(row0 + b) * p.tiles;
-            float m = -INFINITY;
-            for (int t = lane; t < p.tiles; t += 32) m = fmaxf(m, ml[t].x);
+            float m = x0.x;
+            for (int t = lane + 32; t < p.tiles; t += 32) m = fmaxf(m, ml[t].x);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
             double s = 0.0;
             for (int t = lane; t < p.tiles; t += 32) {
-                const float2 x = ml[t];
+                const float2 x = t == lane ? x0 : ml[t];
                 if (x.x > -INFINITY) s += static_cast<double>(x.y) * static_cast<double>(expf(x.x - m));
             }
 #pragma unroll
@@ -432,27 +438,25 @@ __global__ void __launch_bounds__(BS_THREADS) beam_join_kernel(const __grid_cons
         }
     }
     __syncthreads();
-    // A list is a tile's sorted pairs; a finished beam is a list of its one candidate.
-    const int lists = p.beams * p.tiles;
-    auto list_at = [&](int list, int i, u64& key, uint32_t& idx) -> bool {
+    // A list is a tile's sorted pairs; a finished beam is a list of its one candidate.  x: what the tile left in place i.
+    auto pair_of = [&](int list, int i, u64 x, u64& key, uint32_t& idx) -> bool {
         const int b = list / p.tiles, t = list - b * p.tiles;
         if (state[b] == 2) {
             key = key_of(offset[b]);
             idx = static_cast<uint32_t>(b) * p.vocab + p.eos;
             return t == 0 && i == 0;
         }
-        if (state[b] == 0 || i >= p.n_out) return false;
-        const u64 x = p.tile_top[(static_cast<long long>(row0) * p.tiles + list) * p.n_out + i];
-        if (x == 0) return false;
+        if (state[b] == 0 || x == 0) return false;
         key = key_of(static_cast<double>(value_of(static_cast<uint32_t>(x >> 32))) + offset[b]);
         idx = static_cast<uint32_t>(b) * p.vocab + static_cast<uint32_t>(~x);
         return true;
     };
+    auto head_of = [&](int list) { return list == tid ? first : lists_from[static_cast<long long>(list) * p.n_out]; };
     uint32_t mine = 0;
     for (int l = tid; l < lists; l += BS_THREADS) {
         u64 key;
         uint32_t idx;
-        if (list_at(l, 0, key, idx)) mine = max(mine, static_cast<uint32_t>(key >> 32));
+        if (pair_of(l, 0, head_of(l), key, idx)) mine = max(mine, static_cast<uint32_t>(key >> 32));
     }
     const u64 bound = block_bound(mine, p.n_out, reinterpret_cast<uint32_t(*)[32]>(pool.key), sets);
     // the lists whose first pair is not behind the bound, BS_CAP at a time, then their pairs, all of them at once (one after
@@ -464,15 +468,15 @@ __global__ void __launch_bounds__(BS_THREADS) beam_join_kernel(const __grid_cons
             for (int l = l0 + tid; l < min(lists, l0 + BS_CAP); l += BS_THREADS) {
                 u64 key;
                 uint32_t idx;
-                if (list_at(l, 0, key, idx) && !Candidates::before(bk, bi, key, idx)) open[atomicAdd(&n_open, 1u)] = l;
+                if (pair_of(l, 0, head_of(l), key, idx) && !Candidates::before(bk, bi, key, idx)) open[atomicAdd(&n_open, 1u)] = l;
             }
             __syncthreads();
             const int pairs = static_cast<int>(n_open) * p.n_out;
             for (int e = tid; e < pairs; e += BS_THREADS) {
                 u64 key;
                 uint32_t idx;
-                const int l = e / p.n_out;
-                if (list_at(open[l], e - l * p.n_out, key, idx) && !Candidates::before(bk, bi, key, idx)) pool.add(key, idx);
+                const int o = e / p.n_out, i = e - o * p.n_out, l = open[o];
+                if (pair_of(l, i, lists_from[static_cast<long long>(l) * p.n_out + i], key, idx) && !Candidates::before(bk, bi, key, idx)) pool.add(key, idx);
             }
             __syncthreads();
         }
