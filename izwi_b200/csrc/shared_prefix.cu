@@ -760,19 +760,22 @@ Plan make_plan(const izb_ctx* ctx, int64_t groups, int64_t seqs, int kv_heads, i
     Plan pl = {};
     const int64_t rows = seqs * g, sms = ctx && ctx->sm_count > 0 ? ctx->sm_count : 148;
     // Which kernel takes the prefix.  Above 32 rows a second block of 32 would read the tiles again, and the tensor-memory
-    // kernel holds 128 or 256.  Up to 32 its rows are mostly idle, but a 128-token bf16 tile of D = 128 takes it 1,900
-    // cycles against 3,300 to 4,900 here; against that stand some 5 us for an item's first loads, tensor memory and result,
-    // so items have to be long (bf16, 32,768 tokens, 2 x 8 heads: 16 rows 53.8 us against 64.7, 32 rows 54.3 against 73.8;
-    // 12 tiles an item, 5 rows: 118 against 94).  Codes are converted there by warps of their own, which pays from 17 rows:
-    // Q4_0, whose conversion takes most, at any length (4 x 8 beams, 32 rows, 131 own tokens: 1,000 tokens 21.6 us against
-    // 24.5, 4,099 31.5 against 32.9, 8,192 43.1 against 59.1), Int8 for long items (9 tiles an item 32.4 against 30.0, 16 tiles
-    // 47.3 against 47.8, 33 tiles 69.7 against 77.5); with 16 rows 16,384 tokens of Int8 take 52.9 against 48.3.  D = 64: 54 us
-    // against 31 (bf16), 64 against 48 (Int8, 30 rows) at 12 tiles an item.
+    // kernel holds 128 or 256.  Up to 32 its rows are mostly idle, but a tile of 128 tokens of 128 channels takes it less time
+    // (bf16 1,900 cycles against 3,300 to 4,900 here); against that stand some 5 us for an item's first loads, tensor memory
+    // and result, and another 5 to 9 where own tokens follow it, which here fill the same launch.  So its items have to be
+    // long, longer with own tokens.  Microseconds there against here, tiles an item in brackets:
+    //   17 to 32 rows  bf16 20.6/19.6 (9) 31.0/35.5 (16) 51.6/60.4 (32), own tokens 39.6/39.7 (16) 58.8/62.0 (28);
+    //                  Int8 21.4/22.4 (8) 22.2/21.8 (9) 32.2/39.5 (16), own 29.5/26.9 (8) 42.4/42.7 (16);
+    //                  Q4_0, whose conversion takes most, 14.4/15.1 (4) 20.5/22.1 (9), own 22.6/22.4 (4) 27.6/28.4 (8)
+    //   up to 16       bf16 30.5/31.0 (16) 50.9/52.5 (28) 89.2/105.9 (57), own 62.5/53.6 (28) 100.6/107.9 (57);
+    //                  Int8 52.5/48.3 (32), Q4_0 50.1/46.3 (32)
+    // D = 64: 54 against 31 (bf16), 64 against 48 (Int8, 30 rows) at 12 tiles an item.
     const int tc_rows = rows <= TC_ROWS ? TC_ROWS : 2 * TC_ROWS;
     const int64_t tc_items = groups * kv_heads * ((rows + tc_rows - 1) / tc_rows);
     const int tc_chunk = max_prefix > 0 ? choose_chunk(tc_items, max_prefix, sms, 128, 4, 1 << 20) : 0;
-    const int least = rows > 16 ? (quant == IZB_KV_Q4_0 ? 2 : 12) : quant == IZB_KV_NONE ? 16 : 1 << 20;
-    pl.tc = rows > 32 || (head_dim == 128 && tc_chunk >= least * 128);
+    const bool own = max_own > 0;
+    const int least = rows > 16 ? (quant == IZB_KV_NONE ? (own ? 24 : 12) : quant == IZB_KV_INT8 ? (own ? 16 : 10) : own ? 8 : 4) : own ? 48 : 24;
+    pl.tc = rows > 32 || (head_dim == 128 && (rows > 16 || quant == IZB_KV_NONE) && tc_chunk >= least * 128);
     pl.rows = pl.tc ? tc_rows : rows <= 16 ? 16 : 32;
     pl.row_blocks = static_cast<int>((rows + pl.rows - 1) / pl.rows);
     const int64_t slots = (head_dim == 64 && (rows <= 16 || pl.tc) ? 3 : 2) * sms;  // of the other kernel

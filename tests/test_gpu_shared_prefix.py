@@ -257,7 +257,7 @@ def test_agrees_with_paged_attention_over_copies_of_the_prompt(cuda):
 
 
 @pytest.mark.parametrize("quant", ["none", "int8", "q4_0"])
-@pytest.mark.parametrize("seqs,heads,kvh,groups,length", [(8, 16, 4, 1, 60001), (12, 8, 4, 2, 29000), (4, 8, 4, 1, 80000)])
+@pytest.mark.parametrize("seqs,heads,kvh,groups,length", [(8, 16, 4, 1, 60001), (12, 8, 4, 2, 29000), (4, 8, 4, 1, 80000), (4, 8, 4, 1, 116000)])
 def test_long_prefixes_of_few_rows(cuda, quant, seqs, heads, kvh, groups, length):
     """Up to 32 rows over prefixes long enough for the tensor-memory kernel, the last chunk cut anywhere; the definition
     computed on the GPU in 64 bits.  Pages of 24 tokens."""
