@@ -139,7 +139,7 @@ def shared_prefix_attention(q: torch.Tensor, prefix: PagedKvCache, suffix: Paged
     if prefix.page_table.device != dev or (suffix is not None and suffix.page_table.device != dev):
         raise ValueError("shared_prefix_attention: tensors on different devices")
     if out is None:
-        out, out_row = torch.empty((b, h, d), device=dev, dtype=torch.bfloat16), h * d
+        out, out_row = torch.empty_like(q, memory_format=torch.contiguous_format), h * d
     else:
         out_row = out.stride(0)
         if out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != dev or out.stride(2) != 1 or out.stride(1) != d:
