@@ -99,13 +99,27 @@ struct ItemShared {
     long long slot[32];   // per row: its place among the partial results
     float2 wml[4][32];    // per warp and row: maximum and sum
     float factor[4][32];  // per warp and row: weight in the joined result
-    float2 own[SP_MAX_G];  // of an item that finishes its rows: maximum (log2 scale) and sum
+    float2 own[32];        // of an item that does not leave partial results: maximum (log2 scale) and sum of its rows
     int abort_flag;
 };
 
 // Chunks of the prefix a row of `group` has partial results of.
 __device__ __forceinline__ int prefix_chunks_of(const Params& p, int group) {
     return p.prefix.n_chunks ? (length_of(p.prefix, group) + p.prefix.chunk - 1) / p.prefix.chunk : 0;
+}
+
+// Four channels of a row's result.  A row without any token gives zeros; NaN in a sum is not hidden.
+template <int D>
+__device__ __forceinline__ void leave(const Result& to, float4 a, float l, int seq, int head, int col) {
+    const float4 y = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(a.x / l, a.y / l, a.z / l, a.w / l);
+    __nv_bfloat16* out = to.out + seq * to.ld + static_cast<long long>(head) * D + col * 4;
+    const uint32_t lo = izb::pack_bf16x2(y.x, y.y), hi = izb::pack_bf16x2(y.z, y.w);
+    if ((reinterpret_cast<uintptr_t>(out) & 7) == 0) {
+        *reinterpret_cast<uint2*>(out) = make_uint2(lo, hi);
+    } else {
+        const __nv_bfloat162 b[2] = {*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&hi)};
+        out[0] = b[0].x; out[1] = b[0].y; out[2] = b[1].x; out[3] = b[1].y;
+    }
 }
 
 // `a`: weighted values of channels col * 4.. under maximum m (log2 scale) and sum l, joined with the row's partial results
@@ -123,16 +137,42 @@ __device__ __forceinline__ void finish(const Params& p, const Result& to, float4
         m = n;
         a = make_float4(a.x * f + v.x * g, a.y * f + v.y * g, a.z * f + v.z * g, a.w * f + v.w * g);
     }
-    // a row without any token gives zeros; NaN in a sum is not hidden
-    const float4 y = l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(a.x / l, a.y / l, a.z / l, a.w / l);
-    __nv_bfloat16* out = to.out + seq * to.ld + static_cast<long long>(head) * D + col * 4;
-    const uint32_t lo = izb::pack_bf16x2(y.x, y.y), hi = izb::pack_bf16x2(y.z, y.w);
-    if ((reinterpret_cast<uintptr_t>(out) & 7) == 0) {
-        *reinterpret_cast<uint2*>(out) = make_uint2(lo, hi);
-    } else {
-        const __nv_bfloat162 b[2] = {*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&hi)};
-        out[0] = b[0].x; out[1] = b[0].y; out[2] = b[1].x; out[3] = b[1].y;
+    leave<D>(to, a, l, seq, head, col);
+}
+
+// The items of a (group, KV head) lie in a cluster, prefix chunks first: each joins a share of the rows from all of them.
+// 128 threads of every CTA.
+template <int D>
+__device__ __forceinline__ void join_cluster(const Params& p, const Result& to, ItemShared& sh, uint8_t* smem) {
+    const int np = p.prefix.n_chunks, no = p.own.n_chunks, size = np + p.seqs * no;
+    const int rank = static_cast<int>(blockIdx.x) % size, base = static_cast<int>(blockIdx.x) / size;
+    const int group = base / p.kv_heads, kh = base - group * p.kv_heads;
+    const uint32_t own = izb::smem_u32(&sh.own[0]), rows = izb::smem_u32(smem) + p.cluster_rows;
+    izb::cluster_sync_all();
+    for (int i = rank * 128 + static_cast<int>(threadIdx.x); i < p.seqs * p.g * (D / 4); i += size * 128) {
+        const int row = i / (D / 4), col = i % (D / 4), s = row / p.g, h = row - s * p.g;
+        float m = -INFINITY, l = 0.f;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int c = 0; c < np + no; ++c) {
+            const int from = c < np ? c : np + s * no + c - np, r = c < np ? row : h;
+            float2 x;
+            float4 v;
+            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(izb::cluster_map_shared(own + r * 8, from)) : "memory");
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                         : "r"(izb::cluster_map_shared(rows + (r * (D + 4) + col * 4) * 4, from))
+                         : "memory");
+            if (x.x == -INFINITY && x.y == 0.f) continue;  // no token: what lies there is nobody's
+            const float n = fmaxf(m, x.x), u = n == -INFINITY ? 0.f : n;
+            const float f = ex2(m - u), g = ex2(x.x - u);
+            l = l * f + x.y * g;
+            m = n;
+            a = make_float4(a.x * f + v.x * g, a.y * f + v.y * g, a.z * f + v.z * g, a.w * f + v.w * g);
+        }
+        leave<D>(to, a, l, group * p.seqs + s, kh * p.g + h, col);
     }
+    izb::cluster_sync_all();  // nobody leaves while its results are read
 }
 
 // One item: n_rows (at most 16 MT) query rows from row0 that meet KV head kh of `src` row `src_row`, a chunk of tokens from t0.
@@ -141,8 +181,10 @@ __device__ __forceinline__ void finish(const Params& p, const Result& to, float4
 // registers the copying warps do not need go to the computing ones (setmaxnreg; their shares add up to the launch's).
 //   Scores and outputs are mma.sync products of 16 rows: with at most 32 rows a 128-row tensor-memory tile would be idle
 // for three quarters of its rows, while here a tile's fragments are read (or made from codes) exactly once.
-//   FINISH: the item holds all own tokens of its rows and the prefix is done; it leaves the rows' results.
-template <int D, int MT, int Q, int MT_LAUNCH, bool FINISH = false>
+//   PARTS: the chunk's result goes among the partial results.  FINISH: the item holds all own tokens of its rows and the prefix
+// is done; it leaves the rows' results.  CLUSTER: so do together the items of a (group, KV head), which are a cluster.
+enum Mode { PARTS, FINISHES, CLUSTER };
+template <int D, int MT, int Q, int MT_LAUNCH, Mode MODE = PARTS>
 __device__ __forceinline__ void attend(const Params& p, const Source& src, int src_row, int kh, int seq0, int row0, int n_rows, int t0,
                                        int chunk_slot, int chunks_total, uint8_t* smem, ItemShared& sh, const Result& to = Result{}) {
     using L = Layout<D, Q>;
@@ -198,6 +240,7 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
         }
     }
     const int n_tok = min(length_of(src, src_row) - t0, src.chunk);
+    constexpr bool FINISH = MODE == FINISHES;
     const int np = FINISH ? prefix_chunks_of(p, seq0 / p.seqs) : 0;
     if (n_tok <= 0) {
         if (FINISH)
@@ -206,6 +249,10 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
                 finish<D>(p, to, make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f, (static_cast<long long>(seq0) * p.heads + head) * chunks_total, np, seq0, head,
                           i % (D / 4));
             }
+        if (MODE == CLUSTER && tid < 128) {
+            if (tid < n_rows) sh.own[tid] = make_float2(-INFINITY, 0.f);
+            join_cluster<D>(p, to, sh, smem);
+        }
         return;
     }
     const int n_tiles = (n_tok + L::TILE - 1) / L::TILE;
@@ -590,7 +637,7 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
             sh.factor[w][tid] = f;
             sum += f * x.y;
         }
-        if (FINISH) sh.own[tid] = make_float2(top * p.scale_log2, sum);
+        if (MODE != PARTS) sh.own[tid] = make_float2(top * p.scale_log2, sum);
         else p.ml[sh.slot[tid]] = make_float2(top * p.scale_log2, sum);
     }
     izb::named_bar_sync(1, 128);
@@ -605,8 +652,10 @@ __device__ __forceinline__ void attend(const Params& p, const Source& src, int s
             a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
         }
         if constexpr (FINISH) finish<D>(p, to, a, sh.own[r].x, sh.own[r].y, sh.slot[r] - chunk_slot, np, seq0, kh * p.g + r, col);
+        else if constexpr (MODE == CLUSTER) *reinterpret_cast<float4*>(smem + p.cluster_rows + (r * (D + 4) + col * 4) * 4) = a;
         else *reinterpret_cast<float4*>(p.acc + sh.slot[r] * D + col * 4) = a;
     }
+    if constexpr (MODE == CLUSTER) join_cluster<D>(p, to, sh, smem);
 }
 
 template <int D, int MT>
@@ -643,6 +692,30 @@ __global__ void __launch_bounds__(SP_THREADS, Regs<D, MT>::CTAS) shared_prefix_k
     else attend<D, 1, IZB_KV_Q4_0, MT>(p, p.own, seq, kh, seq, 0, p.g, t0, slot, chunks, smem, sh);
 }
 
+// All items of a (group, KV head) in one cluster of up to eight CTAs, which joins their results through shared memory: a call
+// of one launch.
+template <int D, int MT>
+__global__ void __launch_bounds__(SP_THREADS, Regs<D, MT>::CTAS) shared_prefix_cluster_kernel(const __grid_constant__ Params p, const __grid_constant__ Result to) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ ItemShared sh;
+    izb::pdl_launch_dependents();
+    izb::pdl_wait();
+    const int np = p.prefix.n_chunks, no = p.own.n_chunks, size = np + p.seqs * no;
+    const int rank = static_cast<int>(blockIdx.x) % size, base = static_cast<int>(blockIdx.x) / size;
+    const int group = base / p.kv_heads, kh = base - group * p.kv_heads;
+    if (rank < np) {
+        const int t0 = rank * p.prefix.chunk, n = p.seqs * p.g;
+        if (p.prefix.quant == IZB_KV_NONE) attend<D, MT, IZB_KV_NONE, MT, CLUSTER>(p, p.prefix, group, kh, group * p.seqs, 0, n, t0, 0, 0, smem, sh, to);
+        else if (p.prefix.quant == IZB_KV_INT8) attend<D, MT, IZB_KV_INT8, MT, CLUSTER>(p, p.prefix, group, kh, group * p.seqs, 0, n, t0, 0, 0, smem, sh, to);
+        else attend<D, MT, IZB_KV_Q4_0, MT, CLUSTER>(p, p.prefix, group, kh, group * p.seqs, 0, n, t0, 0, 0, smem, sh, to);
+        return;
+    }
+    const int seq = group * p.seqs + (rank - np) / no, t0 = (rank - np) % no * p.own.chunk;
+    if (p.own.quant == IZB_KV_NONE) attend<D, 1, IZB_KV_NONE, MT, CLUSTER>(p, p.own, seq, kh, seq, 0, p.g, t0, 0, 0, smem, sh, to);
+    else if (p.own.quant == IZB_KV_INT8) attend<D, 1, IZB_KV_INT8, MT, CLUSTER>(p, p.own, seq, kh, seq, 0, p.g, t0, 0, 0, smem, sh, to);
+    else attend<D, 1, IZB_KV_Q4_0, MT, CLUSTER>(p, p.own, seq, kh, seq, 0, p.g, t0, 0, 0, smem, sh, to);
+}
+
 // Behind the tensor-memory kernel: an item per (sequence, KV head) takes the sequence's own tokens, joins the chunks of the
 // prefix and leaves the result, where there are few enough own tokens for one item.  (In a launch before it they cost that
 // launch, and this one the reading of their partial results: 64 sequences of up to 256 own tokens 68.7 us against 64.2.)
@@ -654,9 +727,9 @@ __global__ void __launch_bounds__(SP_THREADS, Regs<D, 1>::CTAS) shared_prefix_fi
     izb::pdl_wait();
     const int chunks = p.prefix.n_chunks + p.own.n_chunks;
     const int kh = blockIdx.x % p.kv_heads, seq = blockIdx.x / p.kv_heads;
-    if (p.own.quant == IZB_KV_NONE) attend<D, 1, IZB_KV_NONE, 1, true>(p, p.own, seq, kh, seq, 0, p.g, 0, p.prefix.n_chunks, chunks, smem, sh, to);
-    else if (p.own.quant == IZB_KV_INT8) attend<D, 1, IZB_KV_INT8, 1, true>(p, p.own, seq, kh, seq, 0, p.g, 0, p.prefix.n_chunks, chunks, smem, sh, to);
-    else attend<D, 1, IZB_KV_Q4_0, 1, true>(p, p.own, seq, kh, seq, 0, p.g, 0, p.prefix.n_chunks, chunks, smem, sh, to);
+    if (p.own.quant == IZB_KV_NONE) attend<D, 1, IZB_KV_NONE, 1, FINISHES>(p, p.own, seq, kh, seq, 0, p.g, 0, p.prefix.n_chunks, chunks, smem, sh, to);
+    else if (p.own.quant == IZB_KV_INT8) attend<D, 1, IZB_KV_INT8, 1, FINISHES>(p, p.own, seq, kh, seq, 0, p.g, 0, p.prefix.n_chunks, chunks, smem, sh, to);
+    else attend<D, 1, IZB_KV_Q4_0, 1, FINISHES>(p, p.own, seq, kh, seq, 0, p.g, 0, p.prefix.n_chunks, chunks, smem, sh, to);
 }
 
 // One CTA per (sequence, head): four warps take every fourth chunk, a lane D / 32 channels.
@@ -731,6 +804,7 @@ __global__ void __launch_bounds__(128)
 // ---- host side ---------------------------------------------------------------------------------------------------
 struct Plan {
     bool tc;         // the prefix goes to the tensor-memory kernel
+    bool cluster;    // one launch: the items of a (group, KV head) are a cluster
     bool own_finishes;  // the own tokens are taken behind it, by the launch that joins
     int rows;        // query rows of a prefix item
     int row_blocks;
@@ -789,6 +863,12 @@ Plan make_plan(const izb_ctx* ctx, int64_t groups, int64_t seqs, int kv_heads, i
         pl.own_chunks = static_cast<int>((max_own + pl.own_chunk - 1) / pl.own_chunk);
     }
     pl.own_finishes = pl.tc && pl.own_chunks == 1;
+    // One launch instead of two saves its issue on the host and up to 1 us on the device, as long as all items are resident at
+    // once; clusters of more than two need more room than there is, since they do not fill every place (two launches against
+    // one, us: 160 clusters of two 16.5 / 15.5, 8 of five 6.2 / 6.2 and 13.3 / 11.1 issued by the host, 64 of four 12.2 / 17.0,
+    // 240 of four 16.0 / 23.6).
+    const int64_t size = pl.prefix_chunks + seqs * pl.own_chunks;
+    pl.cluster = !pl.tc && pl.row_blocks == 1 && size > 0 && size <= 8 && groups * kv_heads * size <= (size <= 2 ? slots : sms);
     return pl;
 }
 
@@ -831,8 +911,8 @@ size_t smem_for(const Source& s) {
 }
 
 template <int D, int MT, typename... Args>
-int launch_items(izb_ctx* ctx, cudaStream_t s, void (*kern)(Params, Args...), std::atomic<bool>* ready, size_t smem, int64_t items, const Params& p,
-                 const Args&... args) {
+int launch_items(izb_ctx* ctx, cudaStream_t s, void (*kern)(Params, Args...), std::atomic<bool>* ready, size_t smem, int cluster, int64_t items,
+                 const Params& p, const Args&... args) {
     if (!ready[ctx->device].load(std::memory_order_relaxed)) {
         cudaFuncAttributes attr;
         IZB_CUDA_TRY(cudaFuncGetAttributes(&attr, kern));
@@ -840,7 +920,7 @@ int launch_items(izb_ctx* ctx, cudaStream_t s, void (*kern)(Params, Args...), st
         IZB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ctx->max_smem_optin - static_cast<int>(attr.sharedSizeBytes)));
         ready[ctx->device].store(true, std::memory_order_relaxed);
     }
-    IZB_CUDA_TRY(izb::launch_chained(ctx, kern, dim3(static_cast<unsigned>(items)), dim3(SP_THREADS), smem, s, p, args...));
+    IZB_CUDA_TRY(izb::launch_chained_cluster(ctx, cluster, kern, dim3(static_cast<unsigned>(items)), dim3(SP_THREADS), smem, s, p, args...));
     ctx->launches.fetch_add(1, std::memory_order_relaxed);
     return IZB_OK;
 }
@@ -849,12 +929,35 @@ template <int D, int MT>
 int launch_all_items(izb_ctx* ctx, cudaStream_t s, const Params& p, int64_t items) {
     static std::atomic<bool> ready[IZB_MAX_DEVICES];
     const size_t prefix = p.prefix_items > 0 ? smem_for<D, MT>(p.prefix) : 0, own = smem_for<D, 1>(p.own);
-    return launch_items<D, MT>(ctx, s, shared_prefix_kernel<D, MT>, ready, prefix > own ? prefix : own, items, p);
+    return launch_items<D, MT>(ctx, s, shared_prefix_kernel<D, MT>, ready, prefix > own ? prefix : own, 1, items, p);
+}
+
+// Where an item's exchange between its warps ends.
+template <int D, int MT>
+size_t exchange_end(const Source& s) {
+    if (s.n_chunks == 0) return 0;
+    const int q = s.quant, ld = q == IZB_KV_NONE ? Layout<D, IZB_KV_NONE>::EX_LD : Layout<D, IZB_KV_INT8>::EX_LD;
+    return 16 * MT * D * 2 + s.chunk * 4 + (q == IZB_KV_INT8 ? s.chunk * 4 : 0) + 4 * 16 * MT * ld * 4;
+}
+
+template <int D, int MT>
+int launch_cluster(izb_ctx* ctx, cudaStream_t s, Params p, int64_t groups, __nv_bfloat16* out, long long ld_out) {
+    static std::atomic<bool> ready[IZB_MAX_DEVICES];
+    // the rows' results lie at the end, where the tiles have been and no exchange reaches
+    const size_t rows = 16 * MT * (D + 4) * 4;
+    const size_t sizes[4] = {smem_for<D, MT>(p.prefix), smem_for<D, 1>(p.own), exchange_end<D, MT>(p.prefix) + rows, exchange_end<D, 1>(p.own) + rows};
+    size_t smem = 0;
+    for (size_t x : sizes) smem = x > smem ? x : smem;
+    smem = (smem + 15) / 16 * 16;
+    p.cluster_rows = static_cast<int>(smem - rows);
+    const int size = p.prefix.n_chunks + p.seqs * p.own.n_chunks;
+    return launch_items<D, MT>(ctx, s, shared_prefix_cluster_kernel<D, MT>, ready, smem, size, groups * p.kv_heads * size, p, Result{out, ld_out});
 }
 
 template <int D>
 int launch_dim(izb_ctx* ctx, cudaStream_t s, const Params& p, const Plan& pl, int64_t items, int64_t batch, __nv_bfloat16* out,
                long long ld_out) {
+    if (pl.cluster) return pl.rows == 16 ? launch_cluster<D, 1>(ctx, s, p, batch / p.seqs, out, ld_out) : launch_cluster<D, 2>(ctx, s, p, batch / p.seqs, out, ld_out);
     if (items > 0) {
         const int rc = pl.tc || pl.rows == 16 ? launch_all_items<D, 1>(ctx, s, p, items) : launch_all_items<D, 2>(ctx, s, p, items);
         if (rc != IZB_OK) return rc;
@@ -865,7 +968,7 @@ int launch_dim(izb_ctx* ctx, cudaStream_t s, const Params& p, const Plan& pl, in
     }
     if (pl.own_finishes) {
         static std::atomic<bool> ready[IZB_MAX_DEVICES];
-        return launch_items<D, 1>(ctx, s, shared_prefix_finish_kernel<D>, ready, smem_for<D, 1>(p.own), batch * p.kv_heads, p, Result{out, ld_out});
+        return launch_items<D, 1>(ctx, s, shared_prefix_finish_kernel<D>, ready, smem_for<D, 1>(p.own), 1, batch * p.kv_heads, p, Result{out, ld_out});
     }
     IZB_CUDA_TRY(izb::launch_chained(ctx, shared_prefix_join_kernel<D>, dim3(static_cast<unsigned>(batch * p.heads)), dim3(128), 0, s, p, out,
                                      ld_out));

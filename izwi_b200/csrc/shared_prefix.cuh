@@ -31,6 +31,7 @@ struct Params {
     long long ld_q;
     int seqs, heads, kv_heads, g;  // sequences per group, query heads per KV head
     int row_blocks, prefix_items;
+    int cluster_rows;              // a cluster's items: where in shared memory their rows' results lie
     int* status;
     uint32_t q_sign;   // flips q where the scale is negative, so that the largest product is the largest score
     float scale_log2;  // |scale| / ln 2

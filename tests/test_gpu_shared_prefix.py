@@ -323,16 +323,17 @@ def test_two_graphs_share_a_workspace(cuda):
 
 
 @pytest.mark.parametrize("quant", ["none", "int8", "q4_0"])
-@pytest.mark.parametrize("seqs,heads,slens", [(3, 8, [70, 0, 1]), (11, 8, [70, 0, 1] * 3 + [64, 128]), (11, 8, [900] + [0] * 10), (4, 16, [5] * 4)])
-def test_rows_of_any_stride_and_address(cuda, quant, seqs, heads, slens):
+@pytest.mark.parametrize("seqs,heads,slens,plen", [(3, 8, [70, 0, 1], 1500), (11, 8, [70, 0, 1] * 3 + [64, 128], 1500), (11, 8, [900] + [0] * 10, 1500),
+                                                   (4, 16, [5] * 4, 1500), (3, 8, [70, 0, 1], 100), (7, 8, [9] * 7, 3)])
+def test_rows_of_any_stride_and_address(cuda, quant, seqs, heads, slens, plen):
     """Results two bytes off a word, rows an odd number of elements apart, what lies between them left as it was; few and
-    many rows, own tokens in one item and in several, in the last launch and before it."""
+    many rows, own tokens in one item and in several, in the last launch and before it, all in one cluster."""
     import ctypes as C
 
     from izwi_b200 import _lib as L
     from izwi_b200 import ops, paged
     rng = np.random.default_rng(len(slens))
-    prefix, own = Pool(rng, cuda, [1500], 2, 128, 16, quant), Pool(rng, cuda, slens, 2, 128, 16, quant)
+    prefix, own = Pool(rng, cuda, [plen], 2, 128, 16, quant), Pool(rng, cuda, slens, 2, 128, 16, quant)
     q = torch.from_numpy(rng.normal(0, 1, (seqs, heads, 128)).astype(np.float32)).to(cuda).to(torch.bfloat16)
     want = paged.shared_prefix_attention(q, prefix.cache, own.cache).reshape(seqs, -1)
     p, o, lib, ctx = prefix.cache, own.cache, L.lib(), ops.Context.get(0)
