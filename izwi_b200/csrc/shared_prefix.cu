@@ -10,10 +10,10 @@
 // Work: an item is (group, KV head, block of query rows, chunk of prefix tokens) or (sequence, KV head, chunk of its
 // own tokens); all items go out in one launch, one CTA each, or, with many rows or a long prefix, those of the prefix in
 // a launch of their own on tensor memory (shared_prefix_tc.cu), behind which short own tokens join the last launch; a small
-// call is one launch of clusters that join by themselves.  A CTA walks its chunk in tiles with a running maximum and sum per row and leaves (max, sum, weighted values) for a last
-// launch that joins the chunks of every (sequence, head).  fp32 for scores, maxima, sums and accumulators; p is rounded to
-// bf16 for the product with v (half a step: 2^-8 relative at most, independent per token, which is what the bf16 output
-// itself carries).
+// call is one launch of clusters that join by themselves.  A CTA walks its chunk in tiles with a running maximum and sum
+// per row and leaves (max, sum, weighted values) for a last launch that joins the chunks of every (sequence, head).  fp32
+// for scores, maxima, sums and accumulators; p is rounded to bf16 for the product with v (half a step: 2^-8 relative at
+// most, independent per token, which is what the bf16 output itself carries).
 //
 // Measured (device time of the whole call): 8 x 5 beams over 1,500 tokens, 20 heads of 64, bf16 15.5 us = 4.0 TB/s, bound by
 // the ends of its items; 4 x 8 beams over 4,099 + 131 Int8 tokens, 32 / 8 heads of 128 27.1 us, bound by the instructions of
