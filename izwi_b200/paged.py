@@ -126,7 +126,7 @@ def shared_prefix_attention(q: torch.Tensor, prefix: PagedKvCache, suffix: Paged
     """Single-token attention of sequences that share a prompt (izb_shared_prefix_decode_gqa_attention): q
     [groups * n, heads, head_dim] bf16, `prefix` one sequence per group, `suffix` one per row of q, or None.
     Sequence i attends to the whole of prefix i // n and then to its own suffix.  The two bounds (default: what the
-    tables hold) only size the split over the device."""
+    tables hold) size the split over the device; lengths are cut to them."""
     b, h, d = q.shape
     dev, groups, kvh = q.device, prefix.batch, prefix.kv_heads
     q_row, q_head, q_one = q.stride()
