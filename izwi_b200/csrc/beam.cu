@@ -14,7 +14,7 @@ namespace {
 // Inside a row the order is that of the logits, so one pass over them yields, for every tile of a row, the tile's
 // maximum, its sum of exp(x - maximum) and its n_out largest (value, index) pairs; a second launch forms lse_b from
 // the tiles, the totals of the few pairs that are left (in fp64: candidates of different beams are ranked by them),
-// and their order.  32 x 8 rows of 151,936 bf16 logits: 28.9 us with the join (floor 11.9: reading them once), bound by issue
+// and their order.  32 x 8 rows of 151,936 bf16 logits: 27.5 us with the join (floor 11.9: reading them once), bound by issue
 // slots; some 40 instructions for eight logits and 300 a thread for a tile's ends.
 
 constexpr int BS_THREADS = 256;
@@ -77,6 +77,7 @@ __device__ __forceinline__ uint32_t warp_kth(uint32_t x, int k) {
 // close one when k is well below 32 (22 candidates lie above the median of 32 maxima).
 // So the block is cut into 32 groups, or for larger k into two or four sets of 32 smaller ones, and each set answers for its
 // share of k.  Every thread returns the bound.
+template <int THREADS>
 __device__ __forceinline__ u64 block_bound(uint32_t mine, int k, uint32_t (*all)[32], uint32_t (&set)[4]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int sets = k <= 20 ? 1 : k <= 40 ? 2 : 4, share = (k + sets - 1) / sets;
@@ -84,7 +85,7 @@ __device__ __forceinline__ u64 block_bound(uint32_t mine, int k, uint32_t (*all)
     __syncthreads();
     if (warp < sets) {
         uint32_t v = 0;
-        for (int w = warp; w < BS_WARPS; w += sets) v = max(v, all[w][lane]);
+        for (int w = warp; w < THREADS / 32; w += sets) v = max(v, all[w][lane]);
         v = warp_kth(v, share);
         if (lane == 0) set[warp] = v;
     }
@@ -114,9 +115,9 @@ struct Pool {
 };
 // Descending order over the first n entries (n <= CAP).  Up to one entry per thread: each counts the entries in
 // front of it (n broadcast reads, no barrier between them); more: bitonic exchange over the next power of two.
-template <typename P>
+template <int THREADS, typename P>
 __device__ void pool_sort(P& p, int n) {
-    if (n <= BS_THREADS) {
+    if (n <= THREADS) {
         const int i = threadIdx.x;
         const u64 key = i < n ? p.key[i] : 0;
         const uint32_t idx = i < n ? p.index(i) : 0;
@@ -130,13 +131,13 @@ __device__ void pool_sort(P& p, int n) {
         __syncthreads();
         return;
     }
-    int size = 2 * BS_THREADS;
+    int size = 2 * THREADS;
     while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += BS_THREADS) p.put(i, 0, 0xFFFFFFFFu);
+    for (int i = n + threadIdx.x; i < size; i += THREADS) p.put(i, 0, 0xFFFFFFFFu);
     __syncthreads();
     for (int block = 2; block <= size; block <<= 1)
         for (int step = block >> 1; step > 0; step >>= 1) {
-            for (int i = threadIdx.x; i < size / 2; i += BS_THREADS) {
+            for (int i = threadIdx.x; i < size / 2; i += THREADS) {
                 const int a = 2 * i - (i & (step - 1)), b = a + step;
                 const bool down = (a & block) == 0;
                 const u64 ka = p.key[a], kb = p.key[b];
@@ -155,14 +156,14 @@ __device__ void pool_sort(P& p, int n) {
 // at least CAP - k candidates for good.  Then sorts.  Returns the number of sorted entries, at least the k
 // largest if there are that many.  `scan(key, idx)` calls add for every candidate not behind the bound.  The pool's
 // count is zero, and every thread knows it, on the first entry.
-template <typename P, typename Scan>
+template <int THREADS, typename P, typename Scan>
 __device__ int collect(P& p, u64 bound_key, int k, Scan scan) {
     uint32_t bound_idx = 0xFFFFFFFFu;
     for (;;) {
         scan(bound_key, bound_idx);
         __syncthreads();
         const unsigned n = p.count;
-        pool_sort(p, n < P::CAP ? n : P::CAP);
+        pool_sort<THREADS>(p, n < P::CAP ? n : P::CAP);
         if (n <= P::CAP) return static_cast<int>(n);
         bound_key = p.key[k - 1];
         bound_idx = p.index(k - 1);
@@ -229,19 +230,19 @@ __device__ __forceinline__ bool row_counts(const SelectParams& p, int row) {
     return isfinite(p.scores[row]) && !(p.finished && p.finished[row]);
 }
 
-// One CTA per tile of BS_THREADS * NV 16-byte vectors of a row, copied into shared memory, where three
-// short loops look at it (maximum, sum, candidates); a thread works on every BS_THREADS-th vector.  (Held in registers with
+// One CTA per tile of THREADS * NV 16-byte vectors of a row, copied into shared memory, where three
+// short loops look at it (maximum, sum, candidates); a thread works on every THREADS-th vector.  (Held in registers with
 // everything unrolled, the tile made straight-line code that each CTA ran once, at the speed of instruction fetch: 144 us
 // for 32 x 8 rows of 151936 bf16 logits.)  Rows may start anywhere: vectors are cut on 16-byte boundaries of memory; a tile
 // inside its row is one bulk copy, and the ragged ends are read element by element.  Only finite logits count.
-template <typename T, int NV>
-__global__ void __launch_bounds__(BS_THREADS, NV == 8 ? 6 : 8) beam_tile_kernel(const __grid_constant__ SelectParams p) {
-    constexpr int V = 16 / sizeof(T);
+template <typename T, int NV, int THREADS>
+__global__ void __launch_bounds__(THREADS, NV == 2 ? 8 : 6) beam_tile_kernel(const __grid_constant__ SelectParams p) {
+    constexpr int V = 16 / sizeof(T), WARPS = THREADS / 32;
     constexpr float LOG2E = 1.4426950408889634f;
-    __shared__ __align__(128) uint4 tile_s[BS_THREADS * NV];
+    __shared__ __align__(128) uint4 tile_s[THREADS * NV];
     __shared__ Pool<BS_TILE_CAP, true> pool;  // key_of(value) << 32 | ~index
     __shared__ uint32_t sets[4];
-    __shared__ float wm[BS_WARPS], wl[BS_WARPS];
+    __shared__ float wm[WARPS], wl[WARPS];
     __shared__ unsigned long long landed;
     __shared__ int abort_flag;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -258,12 +259,12 @@ __global__ void __launch_bounds__(BS_THREADS, NV == 8 ? 6 : 8) beam_tile_kernel(
     if (!row_counts(p, row)) return;
     const T* base = static_cast<const T*>(p.logits) + static_cast<long long>(row) * p.ld;
     const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
-    const int first = tile * (BS_THREADS * NV) + tid;
-    uint4* mine = tile_s + tid;  // vector i at mine[i * BS_THREADS]
+    const int first = tile * (THREADS * NV) + tid;
+    uint4* mine = tile_s + tid;  // vector i at mine[i * THREADS]
 
-    const long long tile0 = static_cast<long long>(tile) * (BS_THREADS * NV * V) - skew;
+    const long long tile0 = static_cast<long long>(tile) * (THREADS * NV * V) - skew;
     bool ok = true;
-    if (tile0 >= 0 && tile0 + BS_THREADS * NV * V <= p.vocab) {
+    if (tile0 >= 0 && tile0 + THREADS * NV * V <= p.vocab) {
         if (tid == 0) {
             izb::mbar_expect_tx(izb::smem_u32(&landed), sizeof(tile_s));
             izb::bulk_g2s(izb::smem_u32(tile_s), base + tile0, sizeof(tile_s), izb::smem_u32(&landed));
@@ -272,11 +273,11 @@ __global__ void __launch_bounds__(BS_THREADS, NV == 8 ? 6 : 8) beam_tile_kernel(
     } else {
 #pragma unroll 1
         for (int i = 0; i < NV; ++i) {
-            const long long e0 = static_cast<long long>(first + i * BS_THREADS) * V - skew;
+            const long long e0 = static_cast<long long>(first + i * THREADS) * V - skew;
             if (e0 >= 0 && e0 + V <= p.vocab) {
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(izb::smem_u32(mine + i * BS_THREADS)), "l"(base + e0) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(izb::smem_u32(mine + i * THREADS)), "l"(base + e0) : "memory");
             } else {
-                T* w = reinterpret_cast<T*>(mine + i * BS_THREADS);
+                T* w = reinterpret_cast<T*>(mine + i * THREADS);
                 for (int k = 0; k < V; ++k) {
                     const long long e = e0 + k;
                     w[k] = e >= 0 && e < p.vocab ? base[e] : static_cast<T>(-INFINITY);
@@ -289,20 +290,20 @@ __global__ void __launch_bounds__(BS_THREADS, NV == 8 ? 6 : 8) beam_tile_kernel(
     float mx = -INFINITY, vm[NV];  // the largest of each vector
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        vm[i] = largest<T>(mine[i * BS_THREADS]);
+        vm[i] = largest<T>(mine[i * THREADS]);
         mx = fmaxf(mx, vm[i]);
     }
     if (mx == INFINITY) {  // take the infinities out
         mx = -INFINITY;
 #pragma unroll 1
         for (int i = 0; i < NV; ++i) {
-            T* w = reinterpret_cast<T*>(mine + i * BS_THREADS);
+            T* w = reinterpret_cast<T*>(mine + i * THREADS);
             for (int k = 0; k < V; ++k)
                 if (static_cast<float>(w[k]) == INFINITY) w[k] = static_cast<T>(-INFINITY);
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            vm[i] = largest<T>(mine[i * BS_THREADS]);
+            vm[i] = largest<T>(mine[i * THREADS]);
             mx = fmaxf(mx, vm[i]);
         }
     }
@@ -321,15 +322,15 @@ __global__ void __launch_bounds__(BS_THREADS, NV == 8 ? 6 : 8) beam_tile_kernel(
     // A bound of the tile's n_out largest; ties are left to collect().  With up to as many as there are warps, the n_out-th
     // largest of the warps' maxima (n_out warps have a value that is no smaller), else one from every thread's largest.
     u64 bound;
-    if (p.n_out <= BS_WARPS) {
-        const float v = wm[lane % BS_WARPS];
+    if (p.n_out <= WARPS) {
+        const float v = wm[lane % WARPS];
         int rank = 0;
 #pragma unroll
-        for (int j = 0; j < BS_WARPS; ++j) rank += wm[j] > v || (wm[j] == v && j < lane % BS_WARPS);
+        for (int j = 0; j < WARPS; ++j) rank += wm[j] > v || (wm[j] == v && j < lane % WARPS);
         const float b = __shfl_sync(0xFFFFFFFFu, v, __ffs(__ballot_sync(0xFFFFFFFFu, rank == p.n_out - 1)) - 1);
         bound = b > -INFINITY ? static_cast<u64>(key_of(b)) << 32 : 0ull;
     } else {
-        bound = block_bound(mx > -INFINITY ? key_of(mx) : 0u, p.n_out, reinterpret_cast<uint32_t(*)[32]>(pool.key), sets);
+        bound = block_bound<THREADS>(mx > -INFINITY ? key_of(mx) : 0u, p.n_out, reinterpret_cast<uint32_t(*)[32]>(pool.key), sets);
     }
 
     float sum = 0.f;
@@ -339,7 +340,7 @@ __global__ void __launch_bounds__(BS_THREADS, NV == 8 ? 6 : 8) beam_tile_kernel(
 #pragma unroll 4
         for (int i = 0; i < NV; ++i) {
             float x[V];
-            elements<T>(mine[i * BS_THREADS], x);
+            elements<T>(mine[i * THREADS], x);
 #pragma unroll
             for (int k = 0; k < V; k += 2) {
                 const float2 y = fma2(make_float2(x[k], x[k + 1]), make_float2(LOG2E, LOG2E), make_float2(-shift, -shift));
@@ -351,7 +352,7 @@ __global__ void __launch_bounds__(BS_THREADS, NV == 8 ? 6 : 8) beam_tile_kernel(
             sum = 0.f;
 #pragma unroll 1
             for (int i = 0; i < NV; ++i) {
-                const T* w = reinterpret_cast<const T*>(mine + i * BS_THREADS);
+                const T* w = reinterpret_cast<const T*>(mine + i * THREADS);
                 for (int k = 0; k < V; ++k) {
                     const float x = static_cast<float>(w[k]);
                     if (x == x) sum += ex2(fmaf(x, LOG2E, -shift));
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(BS_THREADS, NV == 8 ? 6 : 8) beam_tile_kernel(
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     if (lane == 0) wl[warp] = sum;
-    const int n = collect(pool, bound, p.n_out, [&](u64 bk, uint32_t) {
+    const int n = collect<THREADS>(pool, bound, p.n_out, [&](u64 bk, uint32_t) {
         const float floor_v = bk >> 32 ? value_of(static_cast<uint32_t>(bk >> 32)) : -INFINITY;
         // which vectors hold a candidate, then only those, element by element
         unsigned hits = 0;
@@ -372,11 +373,11 @@ __global__ void __launch_bounds__(BS_THREADS, NV == 8 ? 6 : 8) beam_tile_kernel(
             const int i = __ffs(hits) - 1;
             hits &= hits - 1;
             float x[V];
-            elements<T>(mine[i * BS_THREADS], x);
+            elements<T>(mine[i * THREADS], x);
 #pragma unroll
             for (int k = 0; k < V; ++k)
                 if (x[k] >= floor_v && x[k] > -INFINITY) {
-                    const uint32_t e = static_cast<uint32_t>(first + i * BS_THREADS) * V - skew + k;
+                    const uint32_t e = static_cast<uint32_t>(first + i * THREADS) * V - skew + k;
                     const u64 key = static_cast<u64>(key_of(x[k])) << 32 | static_cast<uint32_t>(~e);
                     if (key >= bk) pool.add(key, 0);
                 }
@@ -384,12 +385,12 @@ __global__ void __launch_bounds__(BS_THREADS, NV == 8 ? 6 : 8) beam_tile_kernel(
     });
     if (tid == 0) {
         float m = -INFINITY, l = 0.f;
-        for (int w = 0; w < BS_WARPS; ++w) m = fmaxf(m, wm[w]);
-        for (int w = 0; w < BS_WARPS; ++w) l += wm[w] > -INFINITY ? wl[w] * ex2((wm[w] - m) * LOG2E) : 0.f;
+        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, wm[w]);
+        for (int w = 0; w < WARPS; ++w) l += wm[w] > -INFINITY ? wl[w] * ex2((wm[w] - m) * LOG2E) : 0.f;
         p.tile_ml[blockIdx.x] = make_float2(m, l);
     }
     u64* out = p.tile_top + static_cast<long long>(blockIdx.x) * p.n_out;
-    for (int i = tid; i < p.n_out; i += BS_THREADS) out[i] = i < n ? pool.key[i] : 0ull;
+    for (int i = tid; i < p.n_out; i += THREADS) out[i] = i < n ? pool.key[i] : 0ull;
 }
 
 // One CTA per group: log-sums of its beams, then the order of what the tiles kept.
@@ -458,10 +459,10 @@ __global__ void __launch_bounds__(BS_THREADS) beam_join_kernel(const __grid_cons
         uint32_t idx;
         if (pair_of(l, 0, head_of(l), key, idx)) mine = max(mine, static_cast<uint32_t>(key >> 32));
     }
-    const u64 bound = block_bound(mine, p.n_out, reinterpret_cast<uint32_t(*)[32]>(pool.key), sets);
+    const u64 bound = block_bound<BS_THREADS>(mine, p.n_out, reinterpret_cast<uint32_t(*)[32]>(pool.key), sets);
     // the lists whose first pair is not behind the bound, BS_CAP at a time, then their pairs, all of them at once (one after
     // the other, list by list, every pair was a trip to memory: 190 us for 64 of 8 x 10 lists)
-    const int n = collect(pool, bound, p.n_out, [&](u64 bk, uint32_t bi) {
+    const int n = collect<BS_THREADS>(pool, bound, p.n_out, [&](u64 bk, uint32_t bi) {
         for (int l0 = 0; l0 < lists; l0 += BS_CAP) {
             if (tid == 0) n_open = 0;
             __syncthreads();
@@ -502,10 +503,11 @@ __global__ void __launch_bounds__(BS_THREADS) beam_join_kernel(const __grid_cons
 
 int dtype_bytes(int dtype) { return dtype == IZB_F32 ? 4 : 2; }
 
-// 16-byte vectors per thread of a tile: eight keep enough loads in flight to stream; two when eight would leave SMs
-// without a tile, so that a few rows spread over the chip.
+// Tiles of 2,048 vectors of 16 bytes, which 128 threads share (what a thread does once a tile then counts half as much as with
+// 256: 32 x 8 rows of 151,936 bf16 logits 27.5 us against 28.9), or of 512 with 256 threads where the large ones would leave
+// SMs without a tile, so that a few rows spread over the chip.
 struct SelectPlan {
-    int nv;
+    int nv;  // vectors per BS_THREADS
     int64_t tiles;
 };
 SelectPlan select_plan(const izb_ctx* ctx, int dtype, int64_t rows, int64_t vocab) {
@@ -522,8 +524,8 @@ size_t select_bytes(const SelectPlan& pl, int64_t rows, int n_out) {
 
 template <typename T>
 cudaError_t launch_tiles(izb_ctx* ctx, cudaStream_t s, const SelectParams& p, int nv, unsigned grid) {
-    if (nv == 8) return izb::launch_chained(ctx, beam_tile_kernel<T, 8>, dim3(grid), dim3(BS_THREADS), 0, s, p);
-    return izb::launch_chained(ctx, beam_tile_kernel<T, 2>, dim3(grid), dim3(BS_THREADS), 0, s, p);
+    if (nv == 8) return izb::launch_chained(ctx, beam_tile_kernel<T, 16, BS_THREADS / 2>, dim3(grid), dim3(BS_THREADS / 2), 0, s, p);
+    return izb::launch_chained(ctx, beam_tile_kernel<T, 2, BS_THREADS>, dim3(grid), dim3(BS_THREADS), 0, s, p);
 }
 
 // ---- reordering of the paged caches --------------------------------------------------------------------------------
