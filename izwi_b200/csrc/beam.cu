@@ -14,7 +14,7 @@ namespace {
 // Inside a row the order is that of the logits, so one pass over them yields, for every tile of a row, the tile's
 // maximum, its sum of exp(x - maximum) and its n_out largest (value, index) pairs; a second launch forms lse_b from
 // the tiles, the totals of the few pairs that are left (in fp64: candidates of different beams are ranked by them),
-// and their order.  32 x 8 rows of 151,936 bf16 logits: 27.5 us with the join (floor 11.9: reading them once), bound by issue
+// and their order.  32 x 8 rows of 151,936 bf16 logits: 26.1 us with the join (floor 11.9: reading them once), bound by issue
 // slots; some 40 instructions for eight logits and 300 a thread for a tile's ends.
 
 constexpr int BS_THREADS = 256;
@@ -236,7 +236,7 @@ __device__ __forceinline__ bool row_counts(const SelectParams& p, int row) {
 // for 32 x 8 rows of 151936 bf16 logits.)  Rows may start anywhere: vectors are cut on 16-byte boundaries of memory; a tile
 // inside its row is one bulk copy, and the ragged ends are read element by element.  Only finite logits count.
 template <typename T, int NV, int THREADS>
-__global__ void __launch_bounds__(THREADS, NV == 2 ? 8 : 6) beam_tile_kernel(const __grid_constant__ SelectParams p) {
+__global__ void __launch_bounds__(THREADS, 8) beam_tile_kernel(const __grid_constant__ SelectParams p) {
     constexpr int V = 16 / sizeof(T), WARPS = THREADS / 32;
     constexpr float LOG2E = 1.4426950408889634f;
     __shared__ __align__(128) uint4 tile_s[THREADS * NV];
@@ -503,19 +503,21 @@ __global__ void __launch_bounds__(BS_THREADS) beam_join_kernel(const __grid_cons
 
 int dtype_bytes(int dtype) { return dtype == IZB_F32 ? 4 : 2; }
 
-// Tiles of 2,048 vectors of 16 bytes, which 128 threads share (what a thread does once a tile then counts half as much as with
-// 256: 32 x 8 rows of 151,936 bf16 logits 27.5 us against 28.9), or of 512 with 256 threads where the large ones would leave
-// SMs without a tile, so that a few rows spread over the chip.
+// Tiles of 1,280 vectors of 16 bytes, ten for each of 128 threads: enough for a thread that what it does once a tile does not
+// show, and eight tiles on an SM (32 x 8 rows of 151,936 bf16 logits: 26.1 us; sixteen vectors 27.4, eight 27.2, eight for each
+// of 256 threads 28.9).  Tiles of 512 with 256 threads where the large ones would leave SMs without one, so that a few rows
+// spread over the chip (4 x 4 rows of 51,865: 9.5 us against 10.1), unless a group's lists become many for the one CTA that
+// joins them (8 rows of 151,936: 304 lists 13.5 us, 120 of the large tiles 9.2).
 struct SelectPlan {
-    int nv;  // vectors per BS_THREADS
+    bool large;
     int64_t tiles;
 };
-SelectPlan select_plan(const izb_ctx* ctx, int dtype, int64_t rows, int64_t vocab) {
+SelectPlan select_plan(const izb_ctx* ctx, int dtype, int64_t groups, int beams, int64_t vocab) {
     const int64_t v = 16 / dtype_bytes(dtype), vectors = (vocab + v - 1 + v - 1) / v;  // a row may start up to v - 1 elements into a vector
+    const int64_t large = (vectors + 1279) / 1280, small = (vectors + 511) / 512;
     SelectPlan pl;
-    const int64_t wide = (vectors + BS_THREADS * 8 - 1) / (BS_THREADS * 8);
-    pl.nv = rows * wide >= (ctx && ctx->sm_count > 0 ? ctx->sm_count : 148) ? 8 : 2;
-    pl.tiles = (vectors + BS_THREADS * pl.nv - 1) / (BS_THREADS * pl.nv);
+    pl.large = groups * beams * large >= (ctx && ctx->sm_count > 0 ? ctx->sm_count : 148) || beams * small > 128;
+    pl.tiles = pl.large ? large : small;
     return pl;
 }
 size_t select_bytes(const SelectPlan& pl, int64_t rows, int n_out) {
@@ -523,9 +525,9 @@ size_t select_bytes(const SelectPlan& pl, int64_t rows, int n_out) {
 }
 
 template <typename T>
-cudaError_t launch_tiles(izb_ctx* ctx, cudaStream_t s, const SelectParams& p, int nv, unsigned grid) {
-    if (nv == 8) return izb::launch_chained(ctx, beam_tile_kernel<T, 16, BS_THREADS / 2>, dim3(grid), dim3(BS_THREADS / 2), 0, s, p);
-    return izb::launch_chained(ctx, beam_tile_kernel<T, 2, BS_THREADS>, dim3(grid), dim3(BS_THREADS), 0, s, p);
+cudaError_t launch_tiles(izb_ctx* ctx, cudaStream_t s, const SelectParams& p, bool large, unsigned grid) {
+    if (large) return izb::launch_chained(ctx, beam_tile_kernel<T, 10, 128>, dim3(grid), dim3(128), 0, s, p);
+    return izb::launch_chained(ctx, beam_tile_kernel<T, 2, 256>, dim3(grid), dim3(256), 0, s, p);
 }
 
 // ---- reordering of the paged caches --------------------------------------------------------------------------------
@@ -822,7 +824,7 @@ size_t izb_beam_select_workspace_bytes(const izb_ctx* ctx, int32_t dtype, int64_
     if (groups <= 0 || beams <= 0 || beams > BS_MAX_BEAMS || vocab <= 0 || vocab > INT32_MAX / beams || n_out <= 0 || n_out > BS_MAX_OUT ||
         groups > INT32_MAX / beams)
         return 0;
-    return select_bytes(select_plan(ctx, dtype, groups * beams, vocab), groups * beams, n_out);
+    return select_bytes(select_plan(ctx, dtype, groups, beams, vocab), groups * beams, n_out);
 }
 
 int32_t izb_beam_select(izb_ctx* ctx, izb_stream stream, const void* logits, int32_t dtype, int64_t groups, int32_t beams, int64_t vocab,
@@ -844,7 +846,7 @@ int32_t izb_beam_select(izb_ctx* ctx, izb_stream stream, const void* logits, int
     if (same_scores ? n_out != beams : (scores_out < scores + rows && scores < scores_out + outs)) return IZB_ERR_BAD_ARG;
     if (finished && finished_out && (same_marks ? n_out != beams : (finished_out < finished + rows && finished < finished_out + outs)))
         return IZB_ERR_BAD_ARG;
-    const SelectPlan pl = select_plan(ctx, dtype, rows, vocab);
+    const SelectPlan pl = select_plan(ctx, dtype, groups, beams, vocab);
     if (rows > INT32_MAX / pl.tiles) return IZB_ERR_UNSUPPORTED;
     const size_t need = select_bytes(pl, rows, n_out);
     if (!workspace || workspace_bytes < need || !izb_aligned(workspace, 8)) return IZB_ERR_BAD_ARG;
@@ -869,9 +871,9 @@ int32_t izb_beam_select(izb_ctx* ctx, izb_stream stream, const void* logits, int
     if (!guard.ok) return IZB_ERR_LAUNCH;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const unsigned grid = static_cast<unsigned>(rows * pl.tiles);
-    if (dtype == IZB_F32) IZB_CUDA_TRY(launch_tiles<float>(ctx, s, p, pl.nv, grid));
-    else if (dtype == IZB_F16) IZB_CUDA_TRY(launch_tiles<__half>(ctx, s, p, pl.nv, grid));
-    else IZB_CUDA_TRY(launch_tiles<__nv_bfloat16>(ctx, s, p, pl.nv, grid));
+    if (dtype == IZB_F32) IZB_CUDA_TRY(launch_tiles<float>(ctx, s, p, pl.large, grid));
+    else if (dtype == IZB_F16) IZB_CUDA_TRY(launch_tiles<__half>(ctx, s, p, pl.large, grid));
+    else IZB_CUDA_TRY(launch_tiles<__nv_bfloat16>(ctx, s, p, pl.large, grid));
     IZB_CUDA_TRY(izb::launch_chained(ctx, beam_join_kernel, dim3(static_cast<unsigned>(groups)), dim3(BS_THREADS), 0, s, p));
     ctx->launches.fetch_add(2, std::memory_order_relaxed);
     return IZB_OK;
