@@ -14,8 +14,8 @@ namespace {
 // Inside a row the order is that of the logits, so one pass over them yields, for every tile of a row, the tile's
 // maximum, its sum of exp(x - maximum) and its n_out largest (value, index) pairs; a second launch forms lse_b from
 // the tiles, the totals of the few pairs that are left (in fp64: candidates of different beams are ranked by them),
-// and their order.  32 x 8 rows of 151,936 bf16 logits: 26.1 us with the join (floor 11.9: reading them once), bound by issue
-// slots; some 40 instructions for eight logits and 300 a thread for a tile's ends.
+// and their order.  32 x 8 rows of 151,936 bf16 logits: 26.1 us with the join (floor 11.9: reading them once), bound by
+// the waits between a tile's three loops.
 
 constexpr int BS_THREADS = 256;
 constexpr int BS_WARPS = BS_THREADS / 32;
