@@ -348,16 +348,17 @@ def test_rows_of_any_stride_and_address(cuda, quant, seqs, heads, slens, plen):
     assert torch.equal(got[:, :-3], want) and (got[:, -3:] == 7).all() and room[0] == 7
 
 
+@pytest.mark.parametrize("seqs", [2, 20])
 @pytest.mark.parametrize("quant", ["none", "int8", "q4_0"])
-def test_many_rows_without_prefix_or_without_own_tokens(cuda, quant):
+def test_without_prefix_or_without_own_tokens(cuda, quant, seqs):
     """Bounds of zero leave a cache out, whatever its lengths say; with both at zero every row is zero."""
     from izwi_b200 import ops, paged
     rng = np.random.default_rng(41)
-    prefix, own = Pool(rng, cuda, [70, 3], 2, 64, 16, quant), Pool(rng, cuda, [1, 0, 130, 17] * 10, 2, 64, 16, quant)
+    prefix, own = Pool(rng, cuda, [70, 3], 2, 64, 16, quant), Pool(rng, cuda, ([1, 0, 130, 17] * 10)[:2 * seqs], 2, 64, 16, quant)
     none = Pool(rng, cuda, [0, 0], 2, 64, 16, quant)
     none.cache = prefix.cache
-    check(rng, cuda, 20, 8, none, own, max_prefix_len=0)
-    q = torch.from_numpy(rng.normal(0, 1, (40, 8, 64)).astype(np.float32)).to(cuda).to(torch.bfloat16)
+    check(rng, cuda, seqs, 8, none, own, max_prefix_len=0)
+    q = torch.from_numpy(rng.normal(0, 1, (2 * seqs, 8, 64)).astype(np.float32)).to(cuda).to(torch.bfloat16)
     assert torch.equal(paged.shared_prefix_attention(q, prefix.cache, own.cache, max_seq_len=0), paged.shared_prefix_attention(q, prefix.cache, None))
     assert (paged.shared_prefix_attention(q, prefix.cache, own.cache, max_prefix_len=0, max_seq_len=0) == 0).all()
     ops.Context.get(0).check()
